@@ -9,7 +9,7 @@ The cache: pages of `page` tokens.  Of every token and key/value head, groups of
 minimum (f16 each, `params[page, head, token, group, (scale, minimum)]`); a channel stands for scale * code + minimum.
 Codes are 4 bits, the lower channel of a pair in the low bits of its byte.  Keys lie as
 `k_codes[page, head, token, q, s, byte]` with channel 32 s + 8 q + 2 byte (+ 1), values as
-`v_codes[page, head, token / 16, octet, token % 16, byte]` with channel 8 octet + 2 byte (+ 1).
+`v_codes[page, head, token / 16, column, token % 16, byte]` with channel column + 16 (2 byte (+ 1)).
 """
 import functools
 import math
@@ -142,7 +142,7 @@ def _offsets(lengths):
 def _pools(case, pages, g=None):
     """Codes and parameters of a cache: of an empty one, or (with a generator) of one full of values."""
     kv, dim, page, groups = case["kv"], case["dim"], case["page"], case["dim"] // case["group"]
-    shapes = (pages, kv, page, 4, dim // 32, 4), (pages, kv, page // 16, dim // 8, 16, 4)
+    shapes = (pages, kv, page, 4, dim // 32, 4), (pages, kv, page // 16, 16, 16, dim // 32)
     p = {}
     for name, shape in zip(("k", "v"), shapes):
         if g is None:
@@ -261,7 +261,7 @@ def _quantise(x, group):
     """Codes [..., groups, group] and parameters [..., groups, 2] of [..., dim] in f32."""
     x = x.unflatten(-1, (-1, group))
     low = x.amin(-1, keepdim=True)
-    scale = ((x.amax(-1, keepdim=True) - low) / 15.0).half().float()
+    scale = ((x.amax(-1, keepdim=True) - low) * (1 / 15)).half().float()
     low = low.half().float()
     codes = torch.where(scale > 0, torch.round((x - low) / scale), 0.0).clamp(0.0, 15.0)
     return codes, torch.cat((scale, low), -1).half(), (codes * scale + low).flatten(-2)
@@ -277,17 +277,18 @@ def _append(s):
     kc, kp, held_k = _quantise(k, c["group"])
     vc, vp, held_v = _quantise(s["v"].float(), c["group"])
     kc, vc = (x.flatten(-2).to(torch.uint8) for x in (kc, vc))
-    kc, vc = (x[..., 0::2] | (x[..., 1::2] << 4) for x in (kc, vc))
+    kc, vc = kc.unflatten(-1, (-1, 2)), vc.unflatten(-1, (-1, 2, 16)).transpose(-1, -2)
+    kc, vc = kc[..., 0] | (kc[..., 1] << 4), vc[..., 0] | (vc[..., 1] << 4)
     s["k_codes"][at, :, off] = kc.unflatten(-1, (dim // 32, 4, 4)).transpose(2, 3)
-    s["v_codes"][at, :, off // 16, :, off % 16] = vc.unflatten(-1, (dim // 8, 4))
+    s["v_codes"][at, :, off // 16, :, off % 16] = vc.transpose(2, 3)
     s["k_params"][at, :, off] = kp
     s["v_params"][at, :, off] = vp
     return [x.to(s["q"].dtype) for x in (q, held_k, held_v)]
 
 
 def _read(codes, params, group):
-    """[sequences, tokens, kv, dim] in f32 of natural-order bytes [sequences, pages, kv, page, dim / 2]."""
-    x = _nibbles(codes).unflatten(-1, (-1, group))
+    """[sequences, tokens, kv, dim] in f32 of codes [sequences, pages, kv, page, dim]."""
+    x = codes.unflatten(-1, (-1, group))
     x = (x * params[..., 0:1].float() + params[..., 1:2].float()).flatten(-2)
     return x.transpose(2, 3).flatten(1, 2)
 
@@ -295,8 +296,9 @@ def _read(codes, params, group):
 def _decode(s):
     c = s["case"]
     t = s["table"].long()
-    k = _read(s["k_codes"][t].transpose(4, 5).flatten(4), s["k_params"][t], c["group"])
-    v = _read(s["v_codes"][t].transpose(4, 5).flatten(5).flatten(3, 4), s["v_params"][t], c["group"])
+    k = _nibbles(s["k_codes"][t].transpose(4, 5).flatten(4))
+    v = _nibbles(s["v_codes"][t].transpose(4, 5).flatten(3, 4)).transpose(4, 5).flatten(4)
+    k, v = _read(k, s["k_params"][t], c["group"]), _read(v, s["v_params"][t], c["group"])
     q = s["q"].float().unflatten(1, (c["kv"], c["g"]))
     x = q @ k.permute(0, 2, 3, 1) * c["dim"] ** -0.5
     inside = torch.arange(x.shape[-1], device=x.device) < s["lengths"][:, None, None, None]
@@ -441,12 +443,12 @@ def exact(case, seed):
     for i, n in enumerate(t["lengths"].tolist()):
         ids = t["table"][i, :(n + case["page"] - 1) // case["page"]].long()
         for h in range(kv):
-            kc = t["k_codes"][ids, h].permute(0, 1, 3, 2, 4).reshape(-1, dim // 2)
-            vc = t["v_codes"][ids, h].permute(0, 1, 3, 2, 4).reshape(-1, dim // 2)
+            kc = _split_bytes(t["k_codes"][ids, h].permute(0, 1, 3, 2, 4).reshape(-1, dim // 2))
+            vc = _split_bytes(t["v_codes"][ids, h].permute(0, 1, 3, 2, 4).reshape(-1, 16, dim // 32)).transpose(1, 2)
             rows = []
             for codes, params in ((kc, t["k_params"]), (vc, t["v_params"])):
                 p = params[ids, h].reshape(-1, dim // group, 2).double()
-                x = _split_bytes(codes).reshape(-1, dim // group, group)
+                x = codes.reshape(-1, dim // group, group)
                 rows.append((x * p[..., :1] + p[..., 1:]).reshape(-1, dim)[:n])
             q = t["q"][i, h * g:(h + 1) * g].double().unsqueeze(1)
             out[i, h * g:(h + 1) * g] = _attend(q, rows[0], rows[1], n - 1, 0).squeeze(1)
