@@ -341,6 +341,109 @@ typedef struct {
 int ohip_qconv2d(ohip_ctx* ctx, const ohip_qconv_desc* d, const void* x, const ohip_weight* w,
                  const int32_t* bias_dev, void* y);
 
+/* ------------------------------------------------------------------ serving
+ * The decoder layer of a language model around the products above: products
+ * with 4-bit weights, a paged cache of keys and values in 4 bits, attention
+ * over whole prompts and of one token over that cache.  No counterpart in
+ * the reference's providers.  All calls are ordered on the context's stream
+ * and can be captured once warm; lengths, offsets, slots and page tables are
+ * device arrays, so that a captured step serves any of their values.  Values
+ * there that name nothing (a slot or page outside the cache, an offset
+ * outside the tokens) are never followed: such a token is not written, such
+ * a page's tokens are not seen. */
+
+/* A weight of 4-bit codes with a scale (and zero point) per group of K:
+ * B[k][n] = scales[n][k / group] * (codes[n][k] - zero_points[n][k / group]).
+ * codes: host [N][blocks][group / 2] bytes, the lower k in the low bits,
+ * blocks = ceil(K / group); scales: host [N][blocks] of `dtype` (F32 / F16 /
+ * BF16), the activations' type; zero_points: host [N][ceil(blocks / 2)] bytes,
+ * the lower block in the low bits, or NULL for 8.  group: 32, 64, 128 or 256. */
+int ohip_weight_q4(ohip_ctx* ctx, const ohip_weight_key* key, const uint8_t* codes, int64_t k, int64_t n, int group,
+                   int dtype, const void* scales, const uint8_t* zero_points, ohip_weight** out);
+/* Y[M,N] = act(A B + bias), B of ohip_weight_q4, A / bias [N] (may be NULL) /
+ * Y of `dtype`.  Up to 64 rows the codes are multiplied as they are (exact
+ * products, f32 sums by group); more rows unpack B to `dtype` (each value
+ * rounded once) into a pool buffer for the MFMA engine. */
+typedef struct {
+    int64_t m, k, n;
+    int dtype;
+    int act;               /* ohip_act */
+    float act_lo, act_hi;
+    int64_t lda, ldy;      /* row strides in elements; 0 = packed */
+} ohip_gemm_q4_desc;
+int ohip_gemm_q4(ohip_ctx* ctx, const ohip_gemm_q4_desc* d, const void* a, const ohip_weight* b, const void* bias,
+                 void* y);
+
+/* A cache of keys and values: `pages` pages of `page` tokens (a multiple of
+ * 16), caller-owned device memory, 16-byte aligned.  Of every token and key
+ * head, `group` channels (32, 64 or 128, a divisor of head_dim) share a scale
+ * and a minimum, f16 pairs params[page][kv_head][token][group][2]; a channel
+ * stands for scale * code + minimum.  The codes lie as the kernels load them:
+ *   k_codes[page][kv_head][token][4 q][head_dim / 32 s][4 bytes]
+ *       byte b: channels 32 s + 8 q + 2 b (low bits) and + 1
+ *   v_codes[page][kv_head][token / 16][16 columns][token % 16][head_dim / 32 bytes]
+ *       byte b: channels column + 32 b (low bits) and column + 32 b + 16
+ * head_dim is 64 or 128. */
+typedef struct {
+    int64_t pages;
+    int page, kv_heads, head_dim, group;
+    void *k_codes, *v_codes, *k_params, *v_params;
+} ohip_kv_cache;
+
+/* Appends `tokens` keys and values to the cache, rotated by position on the
+ * way, and rotates the queries.  Rows are tokens (ld* elements apart, whole
+ * 16-byte chunks) of heads [head_dim] next to each other.  The first `rot`
+ * channels (a multiple of 16) are turned by the angles of row positions[t] of
+ * cos / sin [max_position][rot / 2] (positions outside are taken as the
+ * nearest row): channel i with i + rot / 2, or 2 i with 2 i + 1 if
+ * interleaved; cos == NULL: no rotation.  Token t goes to slot slots[t] =
+ * page * page_size + place; a negative or too large slot is skipped; two
+ * tokens of one call must not share a slot.  Everything is computed in f32;
+ * scale = f16((max - min) / 15) and minimum = f16(min), kept finite (a NaN
+ * makes its group NaN).  q (heads 0: none) and the outputs may be NULL;
+ * k_out / v_out get what the cache stands for (out_held) or the rotated keys
+ * and the values as they came.  dtype: F16 or BF16. */
+typedef struct {
+    int64_t tokens;
+    int dtype, heads, rot, interleaved, out_held;
+    int64_t max_position;
+    int64_t ldq, ldk, ldv, ldq_out, ldk_out, ldv_out;   /* 0 = packed */
+} ohip_kv_append_desc;
+int ohip_kv_append(ohip_ctx* ctx, const ohip_kv_append_desc* d, const ohip_kv_cache* cache, const void* q,
+                   const void* k, const void* v, const int32_t* positions, const float* cos, const float* sin,
+                   const int32_t* slots, void* q_out, void* k_out, void* v_out);
+
+/* Attention of one query token a sequence over the cache: out[b][h] =
+ * softmax(scale * q[b][h] . K) V over tokens max(0, lens[b] - window) ..
+ * lens[b] - 1 (window 0: all) of sequence b, whose token t is in page
+ * table[b][t / page].  Query head h uses key head h / (heads / kv_heads).
+ * A sequence without tokens gets zeros; a length beyond the table's
+ * width * page is that.  F16 or BF16. */
+typedef struct {
+    int64_t batch;
+    int dtype, heads, width, window;   /* width: page table entries a sequence */
+    float scale;                       /* > 0 */
+    int64_t ldq, ldo;                  /* elements between sequences; 0 = packed */
+} ohip_attn_decode_desc;
+int ohip_attn_decode(ohip_ctx* ctx, const ohip_attn_decode_desc* d, const ohip_kv_cache* cache, const void* q,
+                     const int32_t* table, const int32_t* lens, void* out);
+
+/* Attention over packed sequences: sequence i has the query rows cu_q[i] ..
+ * cu_q[i + 1] - 1 and the key rows cu_k[i] .. cu_k[i + 1] - 1 (device arrays
+ * of seqs + 1 ascending offsets).  Its last query stands at its last key:
+ * query i of nq sees (causal) the keys up to i + nk - nq and (window > 0) at
+ * most `window` of the last of these.  A query that sees no key gets zeros.
+ * head_dim: a multiple of 8 up to 128; rows are 16-byte aligned, heads next
+ * to each other.  F16 or BF16. */
+typedef struct {
+    int64_t q_tokens, k_tokens, seqs;
+    int dtype, heads, kv_heads, head_dim, causal, window;
+    float scale;                       /* > 0 */
+    int64_t ldq, ldk, ldv, ldo;        /* elements between tokens; 0 = packed */
+} ohip_attn_prefill_desc;
+int ohip_attn_prefill(ohip_ctx* ctx, const ohip_attn_prefill_desc* d, const void* q, const void* k, const void* v,
+                      const int32_t* cu_q, const int32_t* cu_k, void* out);
+
 /* ------------------------------------------------------------------ device tensors */
 /* A run-scoped device activation (HipDeviceTensor; the DeviceActivation
  * contract of src/session/gpu_activations.rs:117-189 and

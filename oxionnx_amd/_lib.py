@@ -97,6 +97,33 @@ class QConvDesc(ctypes.Structure):
                 ("out_layout", ctypes.c_int), ("out_table", VP), ("in_pitch", I64)]
 
 
+class GemmQ4Desc(ctypes.Structure):
+    _fields_ = [("m", I64), ("k", I64), ("n", I64), ("dtype", ctypes.c_int), ("act", ctypes.c_int),
+                ("act_lo", ctypes.c_float), ("act_hi", ctypes.c_float), ("lda", I64), ("ldy", I64)]
+
+
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("pages", I64), ("page", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("group", ctypes.c_int), ("k_codes", VP), ("v_codes", VP), ("k_params", VP), ("v_params", VP)]
+
+
+class KvAppendDesc(ctypes.Structure):
+    _fields_ = [("tokens", I64), ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("rot", ctypes.c_int),
+                ("interleaved", ctypes.c_int), ("out_held", ctypes.c_int), ("max_position", I64)] + \
+               [(f, I64) for f in ("ldq", "ldk", "ldv", "ldq_out", "ldk_out", "ldv_out")]
+
+
+class AttnDecodeDesc(ctypes.Structure):
+    _fields_ = [("batch", I64), ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("width", ctypes.c_int),
+                ("window", ctypes.c_int), ("scale", ctypes.c_float), ("ldq", I64), ("ldo", I64)]
+
+
+class AttnPrefillDesc(ctypes.Structure):
+    _fields_ = [("q_tokens", I64), ("k_tokens", I64), ("seqs", I64)] + \
+               [(f, ctypes.c_int) for f in ("dtype", "heads", "kv_heads", "head_dim", "causal", "window")] + \
+               [("scale", ctypes.c_float), ("ldq", I64), ("ldk", I64), ("ldv", I64), ("ldo", I64)]
+
+
 class Attr(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("kind", ctypes.c_int), ("i", I64), ("f", ctypes.c_float),
                 ("ints", ctypes.POINTER(I64)), ("n_ints", ctypes.c_int), ("s", ctypes.c_char_p)]
@@ -179,6 +206,12 @@ SIGNATURES = {
     "ohip_conv_transpose_out_dim": (I64, [I64, I64, I64, I64, I64, I64, I64]),
     "ohip_qgemm": (ctypes.c_int, [VP, ctypes.POINTER(QGemmDesc), VP, VP, VP]),
     "ohip_qconv2d": (ctypes.c_int, [VP, ctypes.POINTER(QConvDesc), VP, VP, VP, VP]),
+    "ohip_weight_q4": (ctypes.c_int, [VP, ctypes.POINTER(WeightKey), VP, I64, I64, ctypes.c_int, ctypes.c_int, VP, VP,
+                                      ctypes.POINTER(VP)]),
+    "ohip_gemm_q4": (ctypes.c_int, [VP, ctypes.POINTER(GemmQ4Desc), VP, VP, VP, VP]),
+    "ohip_kv_append": (ctypes.c_int, [VP, ctypes.POINTER(KvAppendDesc), ctypes.POINTER(KvCacheDesc)] + [VP] * 10),
+    "ohip_attn_decode": (ctypes.c_int, [VP, ctypes.POINTER(AttnDecodeDesc), ctypes.POINTER(KvCacheDesc)] + [VP] * 4),
+    "ohip_attn_prefill": (ctypes.c_int, [VP, ctypes.POINTER(AttnPrefillDesc)] + [VP] * 6),
     "ohip_get_counters": (ctypes.c_int, [VP, ctypes.POINTER(Counters)]),
     "ohip_reset_counters": (ctypes.c_int, [VP]),
     "ohip_set_tile_override": (ctypes.c_int, [VP, ctypes.c_int]),

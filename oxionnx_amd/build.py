@@ -20,7 +20,7 @@ LIB = os.path.join(HERE, "libohip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
-SOURCES = [f"contract_{dt}_{part}.hip" for dt in ("i8", "f16", "f32", "bf16") for part in ("dense", "dense_general", "conv", "conv_general", "conv_nhwc")] + ["aux_kernels.hip", "skinny.hip", "nodes.hip", "ops.cpp", "dispatch.cpp"]
+SOURCES = [f"contract_{dt}_{part}.hip" for dt in ("i8", "f16", "f32", "bf16") for part in ("dense", "dense_general", "conv", "conv_general", "conv_nhwc")] + ["aux_kernels.hip", "skinny.hip", "nodes.hip", "q4.hip", "kv_cache.hip", "attention.hip", "ops.cpp", "dispatch.cpp"]
 
 FLAGS = [
     f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
@@ -34,8 +34,10 @@ def _compile(src, incremental=False):
     obj = os.path.join(OUT_DIR, os.path.splitext(src)[0] + ".o")
     if incremental and os.path.exists(obj):
         kern = ["mfma_core.hpp", "launch.hpp", "internal.hpp", "halo_conv.hpp", "norm_stats.hpp"]
-        local = {"ops.cpp": ["internal.hpp", "tile_plan.hpp"], "dispatch.cpp": ["internal.hpp"],
-                 "aux_kernels.hip": kern, "skinny.hip": kern, "nodes.hip": ["internal.hpp", "norm_stats.hpp"]}.get(src, kern + ["contract.inc"])
+        local = {"ops.cpp": ["internal.hpp", "serve.hpp", "tile_plan.hpp"], "dispatch.cpp": ["internal.hpp"],
+                 "aux_kernels.hip": kern, "skinny.hip": kern, "nodes.hip": ["internal.hpp", "norm_stats.hpp"],
+                 "q4.hip": kern + ["serve.hpp"], "kv_cache.hip": ["internal.hpp", "serve.hpp"],
+                 "attention.hip": ["internal.hpp", "serve.hpp"]}.get(src, kern + ["contract.inc"])
         deps = [os.path.join(CSRC, f) for f in [src] + local]
         if src.endswith(".cpp"):
             deps.append(os.path.join(ROOT, "include", "ohip.h"))

@@ -1,0 +1,390 @@
+// The paged cache of keys and values in 4 bits: appending with the position
+// rotation, and attention of one query token a sequence over it.
+#include "serve.hpp"
+
+namespace ohip {
+
+// ------------------------------------------------------------------ append
+// Eight channels a thread, D / 8 threads a head; a row of heads is a token's
+// queries, keys and values.  Rotation, group extremes and codes in f32:
+//   (o1, o2) = (x1 c - x2 s, x2 c + x1 s)          products rounded one by one
+//   scale = f16((max - min) / 15), low = f16(min)  (kept finite)
+//   code = clamp(rint((x - low) / scale), 0, 15)   (a group without extent: 0)
+__device__ __forceinline__ float finite_f16(float v) {
+  return v != v ? v : __builtin_fminf(__builtin_fmaxf(v, -65504.0f), 65504.0f);
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+kv_append_kernel(const KvAppendArgs p) {
+  constexpr int LPH = D / 8;   // lanes a head
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  const int c = threadIdx.x % LPH;
+  const int rows = p.q_heads + 2 * p.kv;
+  const int64_t token = at / rows;
+  const bool live = token < p.tokens;   // whole heads: a head's lanes agree
+  const int slot_head = live ? (int)(at % rows) : 0;
+  const int64_t tk = live ? token : 0;
+  const int kind = slot_head < p.q_heads ? 0 : slot_head < p.q_heads + p.kv ? 1 : 2;   // q, k, v
+  const int h = kind == 0 ? slot_head : kind == 1 ? slot_head - p.q_heads : slot_head - p.q_heads - p.kv;
+  const T* src = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) +
+                 tk * (kind == 0 ? p.ldq : kind == 1 ? p.ldk : p.ldv) + h * D + 8 * c;
+  T raw[8];
+  __builtin_memcpy(raw, __builtin_assume_aligned(src, 16), 16);
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (float)raw[e];
+
+  if (p.cos && kind != 2) {   // (uniform over a head)
+    int64_t pos = p.positions[tk];
+    pos = pos < 0 ? 0 : pos >= p.max_position ? p.max_position - 1 : pos;
+    const float* cs = p.cos + pos * (p.rot / 2);
+    const float* sn = p.sin + pos * (p.rot / 2);
+    if (p.interleaved) {
+      if (8 * c < p.rot) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = x[2 * j], b = x[2 * j + 1], cv = cs[4 * c + j], sv = sn[4 * c + j];
+          x[2 * j] = a * cv - b * sv;
+          x[2 * j + 1] = b * cv + a * sv;
+        }
+      }
+    } else {
+      const int half = p.rot / 16;   // lanes a half of the rotated channels takes
+      const bool low = c < half, in = c < 2 * half;
+      const int mate = (threadIdx.x & 63) + (in ? (low ? half : -half) : 0);
+      const int a0 = 8 * (low ? c : c - half);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float other = __shfl(x[e], mate, 64);
+        if (in) {
+          const float cv = cs[a0 + e], sv = sn[a0 + e];
+          x[e] = low ? x[e] * cv - other * sv : x[e] * cv + other * sv;
+        }
+      }
+    }
+  }
+  T* out = static_cast<T*>(kind == 0 ? p.q_out : kind == 1 ? p.k_out : p.v_out);
+  const int64_t ldo = kind == 0 ? p.ldqo : kind == 1 ? p.ldko : p.ldvo;
+
+  // the group's extremes (NaN is kept: a group with one stands for NaN)
+  float lo = x[0], hi = x[0];
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lo = __builtin_fminf(lo, x[e]);
+    hi = __builtin_fmaxf(hi, x[e]);
+    nan |= x[e] != x[e];
+  }
+  const int gl = p.group / 8;   // lanes a group: 4, 8 or 16, a power of two
+  for (int m = 1; m < gl; m *= 2) {
+    lo = __builtin_fminf(lo, __shfl_xor(lo, m, 64));
+    hi = __builtin_fmaxf(hi, __shfl_xor(hi, m, 64));
+    nan |= __shfl_xor((int)nan, m, 64) != 0;
+  }
+  if (nan) lo = hi = __builtin_nanf("");
+  const _Float16 s16 = (_Float16)finite_f16((hi - lo) * (1.0f / 15.0f)), l16 = (_Float16)finite_f16(lo);
+  const float sc = (float)s16, lw = (float)l16;
+  uint32_t word = 0;   // nibble e: channel 8 c + e
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float v = sc > 0.0f ? __builtin_rintf((x[e] - lw) / sc) : 0.0f;
+    const uint32_t code = v >= 15.0f ? 15u : v > 0.0f ? (uint32_t)v : 0u;
+    word |= code << (4 * e);
+    if (kind != 0 && p.held) x[e] = (float)code * sc + lw;
+  }
+  // a value column holds the channels o + 16 i: nibble i from the lane of channel 16 i + o
+  uint32_t col[16 / LPH];
+#pragma unroll
+  for (int t = 0; t < 16 / LPH; ++t) {
+    const int o = c + t * LPH;
+    col[t] = 0;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const uint32_t w = (uint32_t)__shfl((int)word, (threadIdx.x & 63) - c + 2 * i + (o >> 3), 64);
+      col[t] |= ((w >> (4 * (o & 7))) & 15u) << (4 * i);
+    }
+  }
+  if (!live) return;
+  if (out) {
+    T e8[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) e8[e] = (T)x[e];
+    __builtin_memcpy(__builtin_assume_aligned(out + tk * ldo + h * D + 8 * c, 16), e8, 16);
+  }
+  if (kind == 0) return;
+  const int64_t slot = p.slots[tk];
+  if (slot < 0 || slot >= p.pages * p.page) return;   // a padding token
+  const int64_t page = slot / p.page;
+  const int off = (int)(slot - page * p.page);
+  const int64_t row = (page * p.kv + h) * p.page + off;   // this token's row of the head
+  uint32_t* params = reinterpret_cast<uint32_t*>(kind == 1 ? p.cache_kp : p.cache_vp);
+  if (c % gl == 0)
+    params[row * (D / p.group) + c / gl] =
+        (uint32_t)__builtin_bit_cast(uint16_t, s16) | (uint32_t)__builtin_bit_cast(uint16_t, l16) << 16;
+  if (kind == 1) {
+    // word of channels 32 s + 8 q ..: [q][s]
+    reinterpret_cast<uint32_t*>(p.cache_kc)[row * (D / 8) + (c & 3) * (D / 32) + (c >> 2)] = word;
+  } else {
+    uint8_t* tile = static_cast<uint8_t*>(p.cache_vc) + (row - (off & 15)) * (D / 2);
+#pragma unroll
+    for (int t = 0; t < 16 / LPH; ++t) {
+      const int o = c + t * LPH;
+      uint8_t* to = tile + (o * 16 + (off & 15)) * (D / 32);
+      if constexpr (D == 128) *reinterpret_cast<uint32_t*>(to) = col[t];
+      else *reinterpret_cast<uint16_t*>(to) = (uint16_t)col[t];
+    }
+  }
+}
+
+template <class T> static hipError_t append_t(int dim, const KvAppendArgs& p, hipStream_t st) {
+  const int64_t threads = p.tokens * (p.q_heads + 2 * p.kv) * (dim / 8);
+  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+  if (dim == 128) hipLaunchKernelGGL((kv_append_kernel<T, 128>), grid, block, 0, st, p);
+  else if (dim == 64) hipLaunchKernelGGL((kv_append_kernel<T, 64>), grid, block, 0, st, p);
+  else return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t st) {
+  return dtype == DT_F16 ? append_t<_Float16>(dim, p, st) : dtype == DT_BF16 ? append_t<__bf16>(dim, p, st) : hipErrorInvalidValue;
+}
+
+// ------------------------------------------------------------------ decode
+// One query token a sequence.  With K = s c + m by group, the scores are
+// sum_g s_tg (q_g . c_tg) + m_tg sum(q_g): the matrix instruction multiplies
+// the codes themselves (exact in 16 bits) and the scale meets the f32 sums.
+// The values alike: weights w_tg = p_t s_tg multiply the codes, taken from
+// the middle of their range, c - 8, and sum_t p_t (m_tg + 8 s_tg) is added at
+// the end: over a long context both are sums of either sign that stay as
+// small as the output is.  The bias of the codes' bits goes step by step for
+// the same reason: the step's products start from -136 times its weights.
+// The weights are split in two bf16 parts (16 bits together, f32's range: no
+// scale of the values can make them underflow).
+//
+// A block has the up to 16 query heads of one key head; its waves take steps
+// of 32 tokens.  S^T = K Q^T, lane l = 16 q + h: head h, tokens 4 q + r of
+// two tiles of 16, which is how O^T = V^T P^T wants its right operand when
+// the values' tokens are counted 4 q + j of the first tile, then of the
+// second.
+constexpr int kDecodeWaves = 4;
+
+template <class T, int D, int NG>
+__global__ void __launch_bounds__(64 * kDecodeWaves)
+attn_decode_kernel(const AttnDecodeArgs p) {
+  constexpr int KW = D / 32;   // steps of 32 channels
+  constexpr int CI = D / 16;   // channels of a value column
+  constexpr int SG = KW / NG;  // steps a group
+  constexpr int RS = D + 4;
+  __shared__ float red[kDecodeWaves][16][RS];
+  __shared__ float red_m[kDecodeWaves][16], red_l[kDecodeWaves][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, q = lane >> 4;
+  const int b = blockIdx.y, kvh = blockIdx.x % p.kv, hb = blockIdx.x / p.kv;
+  const int nh = min(16, p.g - hb * 16);   // query heads of this block
+  const int head0 = kvh * p.g + hb * 16;
+  const int64_t room = (int64_t)p.width * p.tpp * 16;
+  const int len = (int)max((int64_t)0, min((int64_t)p.lens[b], room));
+  const int lo = p.window > 0 ? max(0, len - p.window) : 0;
+  const int32_t* table = p.table + (int64_t)b * p.width;
+
+  // the queries' fragments, channels in the codes' order; sums of channels and of bias * channel
+  u32x4 qf[KW];
+  float qs[NG], qb[NG];
+  {
+    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.ldq + (int64_t)(head0 + min(r, nh - 1)) * D;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) qs[g] = qb[g] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KW; ++s) {
+      T e[8], f[8];
+      __builtin_memcpy(e, __builtin_assume_aligned(src + 32 * s + 8 * q, 16), 16);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = r < nh ? e[kCodeOrder[i]] : (T)0.0f;
+        qs[s / SG] += (float)f[i];
+        qb[s / SG] += code_bias<T>(i) * (float)f[i];
+      }
+      __builtin_memcpy(&qf[s], f, 16);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      qs[g] += __shfl_xor(qs[g], 16, 64);
+      qs[g] += __shfl_xor(qs[g], 32, 64);
+      qb[g] += __shfl_xor(qb[g], 16, 64);
+      qb[g] += __shfl_xor(qb[g], 32, 64);
+    }
+  }
+
+  f32x4 o[CI];
+#pragma unroll
+  for (int i = 0; i < CI; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  float om[NG];
+#pragma unroll
+  for (int g = 0; g < NG; ++g) om[g] = 0.0f;
+  float mx = -__builtin_inff(), l = 0.0f;
+  const u32x4 middle = u32x4{0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};   // -136
+
+  const int steps = (len + 31) / 32;
+  for (int st = lo / 32 + wave; st < steps; st += kDecodeWaves) {
+    u32x4 kw[2], vw[2];
+    uint32_t kp[2][4 * NG], vp[2][4 * NG];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int tile = 2 * st + t;
+      if (tile * 16 >= len) tile = 2 * st;   // past the end: any tile that is there
+      int64_t page = table[tile / p.tpp];
+      if (page < 0 || page >= p.pages) page = 0;   // (its tokens are masked below)
+      const int64_t row = (page * p.kv + kvh) * p.tpp * 16 + (int64_t)(tile % p.tpp) * 16;
+      const uint8_t* kc = static_cast<const uint8_t*>(p.cache_kc) + (row + r) * (D / 2) + q * (D / 8);
+      const uint8_t* vc = static_cast<const uint8_t*>(p.cache_vc) + row * (D / 2) + (r * 16 + 4 * q) * (D / 32);
+      __builtin_memcpy(&kw[t], __builtin_assume_aligned(kc, D / 8), D / 8);
+      __builtin_memcpy(&vw[t], __builtin_assume_aligned(vc, D / 8), D / 8);
+      __builtin_memcpy(kp[t], __builtin_assume_aligned(static_cast<const uint32_t*>(p.cache_kp) + (row + 4 * q) * NG, 16), 16 * NG);
+      __builtin_memcpy(vp[t], __builtin_assume_aligned(static_cast<const uint32_t*>(p.cache_vp) + (row + 4 * q) * NG, 16), 16 * NG);
+    }
+    float s[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[t][j] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        f32x4 raw = f32x4{-qb[g], -qb[g], -qb[g], -qb[g]};
+#pragma unroll
+        for (int k = 0; k < SG; ++k) raw = mma16<T>(code_frag<T>(kw[t][g * SG + k]), qf[g * SG + k], raw);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w = kp[t][j * NG + g];
+          s[t][j] = __builtin_fmaf(f16_lo(w), raw[j], s[t][j]);
+          s[t][j] = __builtin_fmaf(f16_hi(w), qs[g], s[t][j]);
+        }
+      }
+    }
+    // tokens outside [lo, len), and of page entries that name no page
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int tile = 2 * st + t;
+      const int64_t page = tile * 16 < len ? table[tile / p.tpp] : 0;
+      const bool there = page >= 0 && page < p.pages;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int token = tile * 16 + 4 * q + j;
+        if (!there || token < lo || token >= len) {
+          s[t][j] = -__builtin_inff();
+#pragma unroll
+          for (int g = 0; g < NG; ++g) vp[t][j * NG + g] = 0;   // whatever is there: 0 * it is 0
+        }
+      }
+    }
+    float m = s[0][0];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = __builtin_fmaxf(m, s[j / 4][j % 4]);
+    m = __builtin_fmaxf(m, __shfl_xor(m, 16, 64));
+    m = __builtin_fmaxf(m, __shfl_xor(m, 32, 64));
+    const float now = __builtin_fmaxf(mx, m);
+    const float base = now == -__builtin_inff() ? 0.0f : now;
+    const float keep = __builtin_amdgcn_exp2f((mx - base) * p.c);
+    mx = now;
+    float pt[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) pt[j] = __builtin_amdgcn_exp2f((s[j / 4][j % 4] - base) * p.c);
+    l *= keep;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l += pt[j];
+    u32x4 hi[NG], lw[NG];
+    f32x4 start[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      om[g] *= keep;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w = vp[j / 4][(j % 4) * NG + g];
+        om[g] = __builtin_fmaf(pt[j], __builtin_fmaf(8.0f, f16_lo(w), f16_hi(w)), om[g]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w0 = pt[2 * j] * f16_lo(vp[j / 2][(2 * j % 4) * NG + g]);
+        const float w1 = pt[2 * j + 1] * f16_lo(vp[j / 2][(2 * j % 4 + 1) * NG + g]);
+        const uint32_t h = pack2<__bf16>(w0, w1);
+        hi[g][j] = h;
+        lw[g][j] = pack2<__bf16>(w0 - bf16_lo(h), w1 - bf16_hi(h));
+      }
+      start[g] = mma16<__bf16>(middle, lw[g], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+      start[g] = mma16<__bf16>(middle, hi[g], start[g]);
+    }
+#pragma unroll
+    for (int i = 0; i < CI; ++i) {
+      u32x4 f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {   // tokens 2 j, 2 j + 1 of the eight
+        uint32_t x;
+        if constexpr (D == 128) {
+          const uint32_t a = vw[j / 2][2 * j % 4], c = vw[j / 2][2 * j % 4 + 1];
+          x = i < 4 ? (a & 0xffffu) | (c << 16) : (a >> 16) | (c & 0xffff0000u);
+        } else {
+          x = vw[j / 2][j % 2];
+        }
+        f[j] = ((x >> (4 * (i % 4))) & 0x000f000fu) | 0x43004300u;
+      }
+      const int g = i * NG / CI;
+      const f32x4 add = mma16<__bf16>(f, hi[g], mma16<__bf16>(f, lw[g], start[g]));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = __builtin_fmaf(o[i][j], keep, add[j]);
+    }
+  }
+  // channel 4 q + j + 16 i of head r; the lanes of a head hold a part each of l and om
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    om[g] += __shfl_xor(om[g], 16, 64);
+    om[g] += __shfl_xor(om[g], 32, 64);
+  }
+#pragma unroll
+  for (int i = 0; i < CI; ++i) {
+    const int g = i * NG / CI;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[wave][r][16 * i + 4 * q + j] = o[i][j] + om[g];
+  }
+  if (q == 0) {
+    red_m[wave][r] = mx;
+    red_l[wave][r] = l;
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < nh * D; idx += 64 * kDecodeWaves) {
+    const int h = idx / D, ch = idx % D;
+    float m = red_m[0][h];
+#pragma unroll
+    for (int w = 1; w < kDecodeWaves; ++w) m = __builtin_fmaxf(m, red_m[w][h]);
+    const float base = m == -__builtin_inff() ? 0.0f : m;
+    float sum = 0.0f, acc = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f((red_m[w][h] - base) * p.c);
+      sum += f * red_l[w][h];
+      acc += f * red[w][h][ch];
+    }
+    static_cast<T*>(p.out)[(int64_t)b * p.ldo + (int64_t)(head0 + h) * D + ch] = (T)(sum == 0.0f ? 0.0f : acc / sum);
+  }
+}
+
+template <class T, int D> static hipError_t decode_d(int group, const AttnDecodeArgs& p, hipStream_t st) {
+  const dim3 grid((unsigned)(p.kv * ((p.g + 15) / 16)), (unsigned)p.batch), block(64 * kDecodeWaves);
+  switch (D / group) {
+    case 1: hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, block, 0, st, p); break;
+    case 2: hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, block, 0, st, p); break;
+    case 4:
+      if constexpr (D == 128) { hipLaunchKernelGGL((attn_decode_kernel<T, D, 4>), grid, block, 0, st, p); break; }
+      [[fallthrough]];
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+hipError_t run_attn_decode(int dtype, int dim, int group, const AttnDecodeArgs& p, hipStream_t st) {
+  if (dim != 64 && dim != 128) return hipErrorInvalidValue;
+  if (dtype == DT_F16) return dim == 64 ? decode_d<_Float16, 64>(group, p, st) : decode_d<_Float16, 128>(group, p, st);
+  if (dtype == DT_BF16) return dim == 64 ? decode_d<__bf16, 64>(group, p, st) : decode_d<__bf16, 128>(group, p, st);
+  return hipErrorInvalidValue;
+}
+
+}  // namespace ohip

@@ -20,6 +20,7 @@
 
 #include "../../include/ohip.h"
 #include "internal.hpp"
+#include "serve.hpp"
 #include "tile_plan.hpp"
 
 using namespace ohip;
@@ -59,7 +60,7 @@ extern "C" int ohip_env_flag(const char* name) {
 }
 
 // ------------------------------------------------------------------ types
-enum WeightKind { WK_GEMM = 1, WK_CONV = 2, WK_QGEMM = 3, WK_QCONV = 4, WK_CONVT = 5 };
+enum WeightKind { WK_GEMM = 1, WK_CONV = 2, WK_QGEMM = 3, WK_QCONV = 4, WK_CONVT = 5, WK_Q4 = 6 };
 
 struct ohip_weight {
   ohip_ctx* ctx = nullptr;
@@ -83,6 +84,9 @@ struct ohip_weight {
   float* comb = nullptr;          // device, rows entries (integer only)
   float comb_a = NAN, comb_y = NAN;
   size_t bytes = 0;
+  int group = 0;                  // 4-bit only: k a scale
+  void* scales = nullptr;         // 4-bit only: of dtype, in the codes' row order
+  uint8_t* zeros = nullptr;       // 4-bit only, null: 8
   // ConvTranspose only: the sub-pixel phase filters (packed like a Conv
   // filter, phase ry * ph_sw + rx) for strides (ph_sh, ph_sw) and pad
   // residues (ph_pt, ph_pl); empty when the gather kernel serves the node.
@@ -342,6 +346,8 @@ static void weight_free(ohip_weight* w) {
   if (w->colsum) (void)hipFree(w->colsum);
   if (w->flip) (void)hipFree(w->flip);
   if (w->comb) (void)hipFree(w->comb);
+  if (w->scales) (void)hipFree(w->scales);
+  if (w->zeros) (void)hipFree(w->zeros);
   delete w;
 }
 
@@ -743,7 +749,7 @@ extern "C" void ohip_weight_release(ohip_weight* w) {
   (void)hipSetDevice(ctx->device);
   // a pooled weight goes back to the stream-ordered pool: work queued after
   // this on the stream may reuse it, so no wait is needed
-  bool pool_only = w->pooled && !w->colsum && !w->flip && !w->comb && w->phases.empty() && !w->ph_all;
+  bool pool_only = w->pooled && !w->colsum && !w->flip && !w->comb && !w->scales && w->phases.empty() && !w->ph_all;
   if (!pool_only) (void)hipStreamSynchronize(ctx->stream);
   weight_free(w);
 }
@@ -2296,6 +2302,271 @@ extern "C" int ohip_qconv2d(ohip_ctx* ctx, const ohip_qconv_desc* d, const void*
     hipError_t e = run_conv_quant(col, wt, col_on_x, o, sc.tile, ctx->stream);
     if (e != hipSuccess) return hip_fail(e, "ohip_qconv2d launch");
   }
+  return OHIP_OK;
+}
+
+// ------------------------------------------------------------------ serving
+// Uploads `bytes` of a host operand into a pool buffer for a packing kernel.
+static int stage_host(ohip_ctx* ctx, const void* host, size_t bytes, void** out) {
+  int rc = pool_alloc(ctx, bytes, out);
+  if (rc) return rc;
+  hipError_t e = hipMemcpyAsync(*out, host, bytes, hipMemcpyHostToDevice, ctx->stream);
+  if (e != hipSuccess) {
+    (void)pool_free(ctx, *out);
+    *out = nullptr;
+    return hip_fail(e, "weight upload");
+  }
+  ctx->counters.weight_uploaded_bytes += bytes;
+  ctx->counters.h2d_bytes += bytes;
+  return OHIP_OK;
+}
+
+extern "C" int ohip_weight_q4(ohip_ctx* ctx, const ohip_weight_key* key, const uint8_t* codes, int64_t k, int64_t n,
+                              int group, int dt, const void* scales, const uint8_t* zero_points, ohip_weight** out) {
+  int rc = activate(ctx);
+  if (rc) return rc;
+  if (!codes || !scales || !out || !is_float(dt) || k <= 0 || n <= 0)
+    return fail(OHIP_E_INVALID, "ohip_weight_q4: bad arguments");
+  if (group != 32 && group != 64 && group != 128 && group != 256)
+    return fail(OHIP_DECLINED, "ohip_weight_q4: groups of 32, 64, 128 or 256");
+  if (k > INT_MAX / 2 || n > INT_MAX / 2 || k > INT64_MAX / 4 / n)
+    return fail(OHIP_DECLINED, "ohip_weight_q4: extent too large");
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  const int64_t blocks = (k + group - 1) / group, rows16 = round_up(n, 16);
+  const size_t src = (size_t)(n * blocks) * (group / 2), src_s = (size_t)(n * blocks) * elem_bytes(dt),
+               src_z = zero_points ? (size_t)(n * ((blocks + 1) / 2)) : 0;
+  const size_t packed = (size_t)rows16 * (size_t)round_up(k, 128) / 2, packed_s = (size_t)(rows16 * blocks) * elem_bytes(dt),
+               packed_z = zero_points ? (size_t)(rows16 * blocks) : 0;
+  // (launches of one thread a word)
+  if (packed / 4 / 256 > INT_MAX || packed_s / 2 / 256 > INT_MAX) return fail(OHIP_DECLINED, "ohip_weight_q4: weight too large");
+  std::string ks = key && key->name ? cache_key(key, WK_Q4, dt, src, {k, n, group, zero_points ? 1 : 0}) : std::string();
+  if (ohip_weight* hit = cache_lookup(ctx, key, ks)) {
+    *out = hit;
+    return OHIP_OK;
+  }
+  auto* w = new (std::nothrow) ohip_weight();
+  if (!w) return fail(OHIP_E_NOMEM, "weight");
+  w->ctx = ctx; w->kind = WK_Q4; w->dtype = dt; w->rows = n; w->k = k; w->group = group;
+  void* stage[3] = {nullptr, nullptr, nullptr};
+  auto done = [&](int code) {
+    for (void* p : stage)
+      if (p) (void)pool_free(ctx, p);
+    if (code) weight_free(w);
+    return code;
+  };
+  if ((rc = stage_host(ctx, codes, src, &stage[0]))) return done(rc);
+  if ((rc = stage_host(ctx, scales, src_s, &stage[1]))) return done(rc);
+  if (zero_points && (rc = stage_host(ctx, zero_points, src_z, &stage[2]))) return done(rc);
+  hipError_t e = dev_malloc(ctx, &w->data, packed);
+  if (e == hipSuccess) e = dev_malloc(ctx, &w->scales, packed_s);
+  if (e == hipSuccess && zero_points) e = dev_malloc(ctx, (void**)&w->zeros, packed_z);
+  if (e != hipSuccess) return done(fail(OHIP_E_NOMEM, std::string("weight hipMalloc: ") + hipGetErrorString(e)));
+  e = run_q4_pack(static_cast<const uint8_t*>(stage[0]), w->data, (int)n, (int)k, group, ctx->stream);
+  if (e == hipSuccess) e = run_q4_pack_rows(elem_bytes(dt), stage[1], w->scales, (int)n, (int)blocks, ctx->stream);
+  if (e == hipSuccess && zero_points) e = run_q4_pack_rows(1, stage[2], w->zeros, (int)n, (int)blocks, ctx->stream);
+  // the caller's host buffers may go away when this returns, and a cached
+  // weight is read by later calls on any stream the caller picks
+  if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+  if (e != hipSuccess) return done(hip_fail(e, "weight packing"));
+  w->bytes = packed + packed_s + packed_z;
+  (void)done(OHIP_OK);
+  return weight_finish(ctx, key, ks, w, out);
+}
+
+extern "C" int ohip_gemm_q4(ohip_ctx* ctx, const ohip_gemm_q4_desc* d, const void* a, const ohip_weight* b,
+                            const void* bias, void* y) {
+  int rc = activate(ctx);
+  if (rc) return rc;
+  if (!d || !b || (d->m > 0 && (!a || !y))) return fail(OHIP_E_INVALID, "ohip_gemm_q4: null argument");
+  if (!is_float(d->dtype) || b->kind != WK_Q4 || b->dtype != d->dtype)
+    return fail(OHIP_E_INVALID, "ohip_gemm_q4: weight kind / dtype mismatch");
+  if (d->k != b->k || d->n != b->rows || d->m < 0)
+    return fail(OHIP_E_SHAPE, "ohip_gemm_q4: shape disagrees with the packed weight");
+  if (d->act < OHIP_ACT_NONE || d->act > OHIP_ACT_LEAKY_RELU) return fail(OHIP_E_INVALID, "ohip_gemm_q4: activation");
+  const int64_t M = d->m, N = d->n, K = d->k;
+  const int64_t lda = d->lda ? d->lda : K, ldy = d->ldy ? d->ldy : N;
+  if (M > 1 && (lda < K || ldy < N)) return fail(OHIP_E_SHAPE, "ohip_gemm_q4: rows overlap");
+  if (M > INT_MAX / 2) return fail(OHIP_DECLINED, "ohip_gemm_q4: extent too large");
+  if (M == 0) return OHIP_OK;
+  const int eb = elem_bytes(d->dtype);
+  if (!aligned(a, eb) || !aligned(y, eb) || (bias && !aligned(bias, eb)))
+    return fail(OHIP_E_INVALID, "ohip_gemm_q4: operands are not aligned to their elements");
+  Q4Args g{a, lda, b->data, b->scales, b->zeros, (int)M, (int)N, (int)K, b->group};
+  if (M > kMaxQ4M) {
+    const int64_t kp = round_up(K, 16 / eb);
+    ohip_weight full;   // the unpacked weight, for this call
+    full.ctx = ctx; full.kind = WK_GEMM; full.dtype = d->dtype; full.rows = N; full.k = K;
+    full.kc = (int)(kp * eb / 16); full.ld_bytes = kp * eb;
+    rc = pool_alloc(ctx, (size_t)(N * kp) * eb, &full.data);
+    if (rc) return rc;
+    hipError_t e;
+    {
+      std::lock_guard<std::mutex> lock(ctx->mu);
+      e = run_q4_unpack(d->dtype, g, full.data, kp, ctx->stream);
+    }
+    if (e != hipSuccess) {
+      rc = hip_fail(e, "ohip_gemm_q4 unpack");
+    } else {
+      ohip_gemm_desc gd{};
+      gd.m = M; gd.k = K; gd.n = N; gd.dtype = d->dtype; gd.alpha = 1.0f; gd.beta = 1.0f;
+      gd.c_kind = bias ? OHIP_C_ROW : OHIP_C_NONE;
+      gd.act = d->act; gd.act_lo = d->act_lo; gd.act_hi = d->act_hi; gd.lda = lda; gd.ldy = ldy;
+      rc = ohip_gemm(ctx, &gd, a, &full, bias, y);
+    }
+    (void)pool_free(ctx, full.data);   // stream-ordered: reused only by later work
+    return rc;
+  }
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  ctx->counters.dispatches++;
+  FloatOut o{};
+  o.y = y; o.si = 1; o.sj = ldy; o.bstride = 0; o.ohw = INT_MAX; o.P = (int)N; o.Q = (int)M;
+  o.vec = (ldy % 4 == 0) && aligned(y, 4 * eb);
+  o.alpha = 1.0f; o.beta = 1.0f; o.bias = bias;
+  o.bias_mode = bias ? BIAS_I : BIAS_NONE;
+  o.act = d->act; o.lo = d->act_lo; o.hi = d->act_hi;
+  if (o.act == ACT_CLIP) {
+    if (std::isnan(o.lo)) o.lo = -INFINITY;
+    if (std::isnan(o.hi)) o.hi = INFINITY;
+    if (!(o.lo <= o.hi)) o.act = ACT_NONE;
+  }
+  ctx->counters.contraction_launches++;
+  hipError_t e = run_gemm_q4(d->dtype, g, o, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "ohip_gemm_q4 launch");
+  return OHIP_OK;
+}
+
+static bool half_type(int dt) { return dt == OHIP_F16 || dt == OHIP_BF16; }
+
+// The cache's own description; `where` names the caller.
+static int cache_check(const ohip_kv_cache* c, const char* where) {
+  const std::string at(where);
+  if (!c || !c->k_codes || !c->v_codes || !c->k_params || !c->v_params)
+    return fail(OHIP_E_INVALID, at + ": null cache");
+  if (c->pages <= 0 || c->page <= 0 || c->kv_heads <= 0) return fail(OHIP_E_SHAPE, at + ": empty cache");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(OHIP_DECLINED, at + ": heads of 64 or 128 channels");
+  if (c->page % 16 != 0) return fail(OHIP_DECLINED, at + ": pages of a multiple of 16 tokens");
+  if ((c->group != 32 && c->group != 64 && c->group != 128) || c->head_dim % c->group != 0)
+    return fail(OHIP_DECLINED, at + ": groups of 32, 64 or 128 channels that divide the head");
+  if (c->pages > (INT64_MAX >> 12) / c->page / c->kv_heads) return fail(OHIP_DECLINED, at + ": cache too large");
+  if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16) || !aligned(c->k_params, 16) || !aligned(c->v_params, 16))
+    return fail(OHIP_E_INVALID, at + ": the cache is not 16-byte aligned");
+  return OHIP_OK;
+}
+
+// Rows of 16-bit elements that the kernels load and store 16 bytes at a time.
+static int rows_check(const void* p, int64_t ld, int64_t width, int64_t rows, const char* where, const char* name) {
+  if (!p) return OHIP_OK;
+  if (ld < 0 || (rows > 1 && ld < width)) return fail(OHIP_E_SHAPE, std::string(where) + ": rows of " + name + " overlap");
+  if (!aligned(p, 16) || (rows > 1 && ld % 8 != 0))
+    return fail(OHIP_DECLINED, std::string(where) + ": rows of " + name + " are not 16-byte aligned");
+  return OHIP_OK;
+}
+
+extern "C" int ohip_kv_append(ohip_ctx* ctx, const ohip_kv_append_desc* d, const ohip_kv_cache* cache, const void* q,
+                              const void* k, const void* v, const int32_t* positions, const float* cosines,
+                              const float* sines, const int32_t* slots, void* q_out, void* k_out, void* v_out) {
+  static const char kWhere[] = "ohip_kv_append";
+  int rc = activate(ctx);
+  if (rc) return rc;
+  if (!d) return fail(OHIP_E_INVALID, "ohip_kv_append: null descriptor");
+  if ((rc = cache_check(cache, kWhere))) return rc;
+  if (!half_type(d->dtype)) return fail(OHIP_DECLINED, "ohip_kv_append: f16 or bf16");
+  if (d->tokens < 0 || d->heads < 0) return fail(OHIP_E_SHAPE, "ohip_kv_append: negative extent");
+  if (d->tokens == 0) return OHIP_OK;
+  if (!k || !v || !slots || (d->heads > 0 && (!q || !q_out)) || (cosines != nullptr) != (sines != nullptr))
+    return fail(OHIP_E_INVALID, "ohip_kv_append: null argument");
+  if (cosines && (!positions || d->max_position <= 0)) return fail(OHIP_E_INVALID, "ohip_kv_append: no positions");
+  if (cosines && (d->rot <= 0 || d->rot > cache->head_dim || d->rot % 16 != 0))
+    return fail(OHIP_DECLINED, "ohip_kv_append: rotated channels: a multiple of 16, at most the head");
+  const int64_t dim = cache->head_dim, wq = d->heads * dim, wk = cache->kv_heads * dim, T = d->tokens;
+  if ((int64_t)d->heads + 2 * (int64_t)cache->kv_heads > INT_MAX / 2 ||
+      T > (int64_t)INT_MAX * 128 / (dim / 8) / (d->heads + 2 * (int64_t)cache->kv_heads))
+    return fail(OHIP_DECLINED, "ohip_kv_append: too many tokens for a launch");
+  KvAppendArgs p{};
+  p.q = d->heads ? q : nullptr; p.k = k; p.v = v;
+  p.q_out = d->heads ? q_out : nullptr; p.k_out = k_out; p.v_out = v_out;
+  p.ldq = d->ldq ? d->ldq : wq; p.ldk = d->ldk ? d->ldk : wk; p.ldv = d->ldv ? d->ldv : wk;
+  p.ldqo = d->ldq_out ? d->ldq_out : wq; p.ldko = d->ldk_out ? d->ldk_out : wk; p.ldvo = d->ldv_out ? d->ldv_out : wk;
+  if ((rc = rows_check(p.q, p.ldq, wq, T, kWhere, "q")) || (rc = rows_check(k, p.ldk, wk, T, kWhere, "k")) ||
+      (rc = rows_check(v, p.ldv, wk, T, kWhere, "v")) || (rc = rows_check(p.q_out, p.ldqo, wq, T, kWhere, "q_out")) ||
+      (rc = rows_check(k_out, p.ldko, wk, T, kWhere, "k_out")) || (rc = rows_check(v_out, p.ldvo, wk, T, kWhere, "v_out")))
+    return rc;
+  p.tokens = T; p.q_heads = d->heads; p.kv = cache->kv_heads; p.group = cache->group;
+  p.rot = d->rot; p.interleaved = d->interleaved; p.held = d->out_held;
+  p.positions = positions; p.cos = cosines; p.sin = sines; p.max_position = d->max_position; p.slots = slots;
+  p.cache_kc = cache->k_codes; p.cache_vc = cache->v_codes; p.cache_kp = cache->k_params; p.cache_vp = cache->v_params;
+  p.pages = cache->pages; p.page = cache->page;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  ctx->counters.dispatches++;
+  hipError_t e = run_kv_append(d->dtype, cache->head_dim, p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "ohip_kv_append launch");
+  return OHIP_OK;
+}
+
+extern "C" int ohip_attn_decode(ohip_ctx* ctx, const ohip_attn_decode_desc* d, const ohip_kv_cache* cache, const void* q,
+                                const int32_t* table, const int32_t* lens, void* out) {
+  static const char kWhere[] = "ohip_attn_decode";
+  int rc = activate(ctx);
+  if (rc) return rc;
+  if (!d) return fail(OHIP_E_INVALID, "ohip_attn_decode: null descriptor");
+  if ((rc = cache_check(cache, kWhere))) return rc;
+  if (!half_type(d->dtype)) return fail(OHIP_DECLINED, "ohip_attn_decode: f16 or bf16");
+  if (d->batch < 0 || d->heads <= 0 || d->width < 0 || d->window < 0 || d->heads % cache->kv_heads != 0)
+    return fail(OHIP_E_SHAPE, "ohip_attn_decode: extents, or heads that the key heads do not divide");
+  if (!(d->scale > 0.0f) || std::isinf(d->scale)) return fail(OHIP_E_INVALID, "ohip_attn_decode: scale");
+  if (d->batch == 0) return OHIP_OK;
+  if (!q || !lens || !out || (d->width > 0 && !table)) return fail(OHIP_E_INVALID, "ohip_attn_decode: null argument");
+  const int64_t w = (int64_t)d->heads * cache->head_dim;
+  if (d->batch > 65535) return fail(OHIP_DECLINED, "ohip_attn_decode: more than 65535 sequences");
+  if ((int64_t)d->width * cache->page > INT_MAX - 64) return fail(OHIP_DECLINED, "ohip_attn_decode: sequences too long");
+  AttnDecodeArgs p{};
+  p.q = q; p.out = out; p.ldq = d->ldq ? d->ldq : w; p.ldo = d->ldo ? d->ldo : w;
+  if ((rc = rows_check(q, p.ldq, w, d->batch, kWhere, "q")) || (rc = rows_check(out, p.ldo, w, d->batch, kWhere, "out")))
+    return rc;
+  p.table = table; p.lens = lens;
+  p.cache_kc = cache->k_codes; p.cache_vc = cache->v_codes; p.cache_kp = cache->k_params; p.cache_vp = cache->v_params;
+  p.pages = cache->pages; p.width = d->width; p.tpp = cache->page / 16;
+  p.batch = (int)d->batch; p.kv = cache->kv_heads; p.g = d->heads / cache->kv_heads; p.window = d->window;
+  p.c = d->scale * 1.4426950408889634f;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  ctx->counters.dispatches++;
+  hipError_t e = run_attn_decode(d->dtype, cache->head_dim, cache->group, p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "ohip_attn_decode launch");
+  return OHIP_OK;
+}
+
+extern "C" int ohip_attn_prefill(ohip_ctx* ctx, const ohip_attn_prefill_desc* d, const void* q, const void* k,
+                                 const void* v, const int32_t* cu_q, const int32_t* cu_k, void* out) {
+  static const char kWhere[] = "ohip_attn_prefill";
+  int rc = activate(ctx);
+  if (rc) return rc;
+  if (!d) return fail(OHIP_E_INVALID, "ohip_attn_prefill: null descriptor");
+  if (!half_type(d->dtype)) return fail(OHIP_DECLINED, "ohip_attn_prefill: f16 or bf16");
+  if (d->q_tokens < 0 || d->k_tokens < 0 || d->seqs < 0 || d->heads <= 0 || d->kv_heads <= 0 || d->window < 0 ||
+      d->head_dim <= 0 || d->heads % d->kv_heads != 0)
+    return fail(OHIP_E_SHAPE, "ohip_attn_prefill: extents, or heads that the key heads do not divide");
+  if (!(d->scale > 0.0f) || std::isinf(d->scale)) return fail(OHIP_E_INVALID, "ohip_attn_prefill: scale");
+  if (d->head_dim % 8 != 0 || d->head_dim > 128)
+    return fail(OHIP_DECLINED, "ohip_attn_prefill: heads of a multiple of 8 channels up to 128");
+  if (d->q_tokens == 0 || d->seqs == 0) return OHIP_OK;
+  if (!q || !out || !cu_q || !cu_k || (d->k_tokens > 0 && (!k || !v)))
+    return fail(OHIP_E_INVALID, "ohip_attn_prefill: null argument");
+  const int64_t wq = (int64_t)d->heads * d->head_dim, wk = (int64_t)d->kv_heads * d->head_dim;
+  if (d->q_tokens > INT_MAX / 4 || d->k_tokens > INT_MAX / 4 || d->seqs > INT_MAX / 4 || d->q_tokens / 128 + d->seqs > 65535)
+    return fail(OHIP_DECLINED, "ohip_attn_prefill: too many tokens for a launch");
+  AttnPrefillArgs p{};
+  p.q = q; p.k = k; p.v = v; p.out = out;
+  p.ldq = d->ldq ? d->ldq : wq; p.ldk = d->ldk ? d->ldk : wk; p.ldv = d->ldv ? d->ldv : wk; p.ldo = d->ldo ? d->ldo : wq;
+  if ((rc = rows_check(q, p.ldq, wq, d->q_tokens, kWhere, "q")) || (rc = rows_check(k, p.ldk, wk, d->k_tokens, kWhere, "k")) ||
+      (rc = rows_check(v, p.ldv, wk, d->k_tokens, kWhere, "v")) || (rc = rows_check(out, p.ldo, wq, d->q_tokens, kWhere, "out")))
+    return rc;
+  p.cu_q = cu_q; p.cu_k = cu_k; p.q_tokens = d->q_tokens; p.k_tokens = d->k_tokens;
+  p.seqs = (int)d->seqs; p.kv = d->kv_heads; p.g = d->heads / d->kv_heads; p.dim = d->head_dim;
+  p.causal = d->causal != 0; p.window = d->window; p.c = d->scale * 1.4426950408889634f;
+  std::lock_guard<std::mutex> lock(ctx->mu);
+  ctx->counters.dispatches++;
+  hipError_t e = run_attn_prefill(d->dtype, p, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "ohip_attn_prefill launch");
   return OHIP_OK;
 }
 

@@ -1,0 +1,298 @@
+// Products with 4-bit weights: Y[m][n] = act(sum_k A[m][k] s[n][k / G] (c[n][k] - z[n][k / G]) + bias[n]),
+// codes c in 0..15, scales s in the activations' type, zero points z in 0..15.
+#include "launch.hpp"
+#include "serve.hpp"
+
+namespace ohip {
+
+// ------------------------------------------------------------------ packing
+// The packed form: tiles of 16 rows (n) by 128 k, each one kilobyte: lane
+// l = 16 q + r of the product's wave finds the codes of row r in its 16 bytes,
+// word s holding k = 32 s + 8 q + e, channel kCodeOrder[i] in nibble order so
+// that code_frag gives e = 0..7 ascending.  Scales and zero points follow the
+// rows: [n / 16][k / G][16].
+__global__ void __launch_bounds__(256)
+q4_pack_kernel(const uint8_t* __restrict__ src, uint32_t* __restrict__ dst, int N, int K, int group, int blocks, int kt,
+               int64_t words) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= words) return;
+  const int s = (int)(i & 3), lane = (int)(i >> 2) & 63;
+  const int64_t tile = i >> 8;
+  const int n = (int)(tile / kt) * 16 + (lane & 15);
+  const int k = (int)(tile % kt) * 128 + 32 * s + 8 * (lane >> 4);
+  uint32_t w = 0;
+  if (n < N) {
+    const uint8_t* row = src + (int64_t)n * blocks * (group / 2);   // a row's blocks lie one after another
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t c = k + e < K ? (row[(k + e) / 2] >> (4 * (e & 1))) & 15u : 0u;
+      // element e of the fragment is nibble (e even: e / 2, odd: 4 + e / 2)
+      w |= c << (4 * ((e >> 1) + 4 * (e & 1)));
+    }
+  }
+  dst[i] = w;
+}
+
+template <class S, class D>
+__global__ void __launch_bounds__(256)
+q4_pack_rows_kernel(const S* __restrict__ src, D* __restrict__ dst, int N, int blocks, int64_t count) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  const int r = (int)(i & 15);
+  const int64_t t = i >> 4;
+  const int n = (int)(t / blocks) * 16 + r, b = (int)(t % blocks);
+  if constexpr (std::is_same<S, uint8_t>::value) {   // zero points: two blocks a byte
+    dst[i] = n < N ? (src[(int64_t)n * ((blocks + 1) / 2) + b / 2] >> (4 * (b & 1))) & 15 : 0;
+  } else {
+    dst[i] = n < N ? src[(int64_t)n * blocks + b] : D(0);
+  }
+}
+
+hipError_t run_q4_pack(const uint8_t* src, void* dst, int N, int K, int group, hipStream_t st) {
+  const int kt = (K + 127) / 128, blocks = (K + group - 1) / group;
+  const int64_t words = (int64_t)((N + 15) / 16) * kt * 256;
+  hipLaunchKernelGGL(q4_pack_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, st, src,
+                     static_cast<uint32_t*>(dst), N, K, group, blocks, kt, words);
+  return hipGetLastError();
+}
+hipError_t run_q4_pack_rows(int elem_bytes, const void* src, void* dst, int N, int blocks, hipStream_t st) {
+  const int64_t count = (int64_t)((N + 15) / 16) * blocks * 16;
+  const dim3 grid((unsigned)((count + 255) / 256)), block(256);
+  if (elem_bytes == 4)
+    hipLaunchKernelGGL((q4_pack_rows_kernel<uint32_t, uint32_t>), grid, block, 0, st, static_cast<const uint32_t*>(src),
+                       static_cast<uint32_t*>(dst), N, blocks, count);
+  else if (elem_bytes == 2)
+    hipLaunchKernelGGL((q4_pack_rows_kernel<uint16_t, uint16_t>), grid, block, 0, st, static_cast<const uint16_t*>(src),
+                       static_cast<uint16_t*>(dst), N, blocks, count);
+  else
+    hipLaunchKernelGGL((q4_pack_rows_kernel<uint8_t, uint8_t>), grid, block, 0, st, static_cast<const uint8_t*>(src),
+                       static_cast<uint8_t*>(dst), N, blocks, count);
+  return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ few rows
+// Eight activations of a lane: a fragment of 16-bit elements, or f32.
+template <class T> struct Act { u32x4 v; };
+template <> struct Act<float> { float v[8]; };
+
+// The sixteen-column product of one word of codes with activations, exact
+// codes: f16 takes the bias off each code (exact); bf16 adds a second product
+// with -(bias + z); f32 runs the f32 instruction, element e of every lane a
+// k of its own.
+template <class T> struct Q4Mma;
+template <> struct Q4Mma<_Float16> {
+  u32x4 off;   // (1024 + z) twice, (64 + z) twice
+  __device__ __forceinline__ void zero(int z) {
+    const _Float16 a = (_Float16)(1024 + z), b = (_Float16)(64 + z);
+    const f16x8 v = {a, a, b, b, a, a, b, b};
+    off = __builtin_bit_cast(u32x4, v);
+  }
+  __device__ __forceinline__ u32x4 frag(uint32_t w) const {
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, code_frag<_Float16>(w)) - __builtin_bit_cast(f16x8, off));
+  }
+  __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<_Float16>& a, f32x4 c) const { return mma16<_Float16>(f, a.v, c); }
+};
+template <> struct Q4Mma<__bf16> {
+  u32x4 off;
+  __device__ __forceinline__ void zero(int z) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, (float)-(128 + z)) >> 16;
+    off = u32x4{b * 0x10001u, b * 0x10001u, b * 0x10001u, b * 0x10001u};
+  }
+  __device__ __forceinline__ u32x4 frag(uint32_t w) const { return code_frag<__bf16>(w); }
+  __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const {
+    return mma16<__bf16>(f, a.v, mma16<__bf16>(off, a.v, c));
+  }
+};
+template <> struct Q4Mma<float> {
+  int z;
+  struct Frag { float v[8]; };
+  __device__ __forceinline__ void zero(int zp) { z = zp; }
+  __device__ __forceinline__ Frag frag(uint32_t w) const {
+    Frag f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f.v[e] = (float)((int)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z);
+    return f;
+  }
+  __device__ __forceinline__ f32x4 mma(const Frag& f, const Act<float>& a, f32x4 c) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(f.v[e], a.v[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+constexpr int kQ4Waves = 8;
+
+// A block takes 16 rows of the weight; its eight waves split K and meet in
+// LDS in wave order.  GS: steps of 32 k a group holds (four for any larger).
+template <class T, int TM, int GS>
+__global__ void __launch_bounds__(64 * kQ4Waves)
+q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes, const T* __restrict__ scales,
+          const uint8_t* __restrict__ zp, int M, int N, int K, int group, const FloatEpi<T> epi) {
+  __shared__ f32x4 red[kQ4Waves][TM][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, q = lane >> 4;
+  const int KT = (K + 127) / 128, blocks = (K + group - 1) / group;
+  const int per = (KT + kQ4Waves - 1) / kQ4Waves;
+  const int t0 = wave * per, t1 = min(t0 + per, KT);
+  const u32x4* wt = codes + (int64_t)blockIdx.x * KT * 64 + lane;
+  const T* sc = scales + (int64_t)blockIdx.x * blocks * 16;
+  const uint8_t* zr = zp ? zp + (int64_t)blockIdx.x * blocks * 16 : nullptr;
+  const T* ar[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) ar[t] = a + (int64_t)min(t * 16 + r, M - 1) * lda;
+  f32x4 acc[TM];
+#pragma unroll
+  for (int t = 0; t < TM; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int kt = t0; kt < t1; ++kt) {
+    const u32x4 w = wt[(int64_t)kt * 64];
+    f32x4 raw[TM];
+    Q4Mma<T> mul;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = kt * 128 + s * 32 + 8 * q;
+      const int b = min((kt * 128 + s * 32) / group, blocks - 1);
+      if (s % GS == 0) {
+        mul.zero(zr ? zr[(int64_t)b * 16 + r] : 8);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) raw[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+      const auto f = mul.frag(w[s]);
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+        Act<T> x;
+        if (k + 8 <= K && t * 16 + r < M) {
+          __builtin_memcpy(&x, ar[t] + k, sizeof(x));
+        } else {
+          T e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = t * 16 + r < M && k + i < K ? ar[t][k + i] : T(0);
+          __builtin_memcpy(&x, e, sizeof(x));
+        }
+        raw[t] = mul.mma(f, x, raw[t]);
+      }
+      if (s % GS == GS - 1) {
+        f32x4 sv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sv[i] = to_f32(sc[(int64_t)b * 16 + 4 * q + i]);
+#pragma unroll
+        for (int t = 0; t < TM; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(sv[i], raw[t][i], acc[t][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TM; ++t) red[wave][t][lane] = acc[t];
+  __syncthreads();
+  if (wave >= TM) return;
+  f32x4 v = red[0][wave][lane];
+#pragma unroll
+  for (int k = 1; k < kQ4Waves; ++k) v += red[k][wave][lane];
+  const int i = blockIdx.x * 16 + 4 * q, j = wave * 16 + r;
+  if (j >= M || i >= N) return;
+  typename FloatEpi<T>::PreI pi;
+  typename FloatEpi<T>::PreJ pj;
+  epi.load_i(pi, i);
+  epi.load_j(pj, j);
+  uint32_t bits[4];
+  epi.finish(pi, pj, i, j, v, bits);
+  const OutAddr out = epi.addr();
+  store_group(out, epi.out_bytes(), out.row(i), i, j, bits);
+}
+
+template <class T, int TM>
+static hipError_t q4_t(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
+  const T* a = static_cast<const T*>(g.a);
+  const u32x4* codes = static_cast<const u32x4*>(g.codes);
+  const T* sc = static_cast<const T*>(g.scales);
+  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * kQ4Waves);
+  if (g.group == 32)
+    hipLaunchKernelGGL((q4_kernel<T, TM, 1>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+  else if (g.group == 64)
+    hipLaunchKernelGGL((q4_kernel<T, TM, 2>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+  else
+    hipLaunchKernelGGL((q4_kernel<T, TM, 4>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+  return hipGetLastError();
+}
+
+template <class T> static hipError_t q4_m(const Q4Args& g, const FloatOut& o, hipStream_t st) {
+  const FloatEpi<T> epi = make_float_epi<T>(o);
+  if (g.M <= 16) return q4_t<T, 1>(g, epi, st);
+  if (g.M <= 32) return q4_t<T, 2>(g, epi, st);
+  if (g.M <= kMaxQ4M) return q4_t<T, 4>(g, epi, st);
+  return hipErrorInvalidValue;
+}
+
+hipError_t run_gemm_q4(int dtype, const Q4Args& g, const FloatOut& o, hipStream_t st) {
+  switch (dtype) {
+    case DT_F32: return q4_m<float>(g, o, st);
+    case DT_F16: return q4_m<_Float16>(g, o, st);
+    case DT_BF16: return q4_m<__bf16>(g, o, st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+// ------------------------------------------------------------------ many rows
+// The weight as K-contiguous rows of T (ldw elements, zeros past K) for the
+// MFMA engine: s * (c - z) in f32, rounded once.
+template <class T>
+__global__ void __launch_bounds__(256)
+q4_unpack_kernel(const u32x4* __restrict__ codes, const T* __restrict__ scales, const uint8_t* __restrict__ zp,
+                 T* __restrict__ dst, int N, int K, int64_t ldw, int group, int kt, int64_t tiles) {
+  const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tile >= tiles) return;
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int64_t n16 = tile / kt;
+  const int k0 = (int)(tile % kt) * 128, blocks = (K + group - 1) / group;
+  const int64_t n = n16 * 16 + r;
+  if (n >= N) return;
+  const u32x4 w = codes[tile * 64 + lane];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    const int k = k0 + 32 * s + 8 * q;
+    if (k >= ldw) continue;
+    const int64_t b = (n16 * blocks + min((k0 + 32 * s) / group, blocks - 1)) * 16 + r;
+    const float sv = to_f32(scales[b]);
+    const int z = zp ? zp[b] : 8;
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int c = (int)((w[s] >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z;
+      e[i] = k + i < K ? from_f32<T>(sv * (float)c) : from_f32<T>(0.0f);
+    }
+    T* to = dst + n * ldw + k;
+    if (k + 8 <= ldw) {
+      __builtin_memcpy(__builtin_assume_aligned(to, 16), e, sizeof(e));
+    } else {   // rows of a whole number of 16-byte chunks: f32 may end in half of the eight
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < ldw) to[i] = e[i];
+    }
+  }
+}
+
+hipError_t run_q4_unpack(int dtype, const Q4Args& g, void* dst, int64_t ldw, hipStream_t st) {
+  const int kt = (g.K + 127) / 128;
+  const int64_t tiles = (int64_t)((g.N + 15) / 16) * kt;
+  const dim3 grid((unsigned)((tiles + 3) / 4)), block(256);
+  const u32x4* codes = static_cast<const u32x4*>(g.codes);
+  switch (dtype) {
+    case DT_F32:
+      hipLaunchKernelGGL((q4_unpack_kernel<float>), grid, block, 0, st, codes, static_cast<const float*>(g.scales), g.zp,
+                         static_cast<float*>(dst), g.N, g.K, ldw, g.group, kt, tiles);
+      break;
+    case DT_F16:
+      hipLaunchKernelGGL((q4_unpack_kernel<_Float16>), grid, block, 0, st, codes, static_cast<const _Float16*>(g.scales),
+                         g.zp, static_cast<_Float16*>(dst), g.N, g.K, ldw, g.group, kt, tiles);
+      break;
+    case DT_BF16:
+      hipLaunchKernelGGL((q4_unpack_kernel<__bf16>), grid, block, 0, st, codes, static_cast<const __bf16*>(g.scales),
+                         g.zp, static_cast<__bf16*>(dst), g.N, g.K, ldw, g.group, kt, tiles);
+      break;
+    default: return hipErrorInvalidValue;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace ohip

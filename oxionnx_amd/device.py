@@ -60,6 +60,11 @@ _CONV = _Packer("@16q4i2fi0q", L.ConvDesc)
 _CONVT = _Packer("@18qi0q", L.ConvTDesc)
 _MATMUL = _Packer("@6qi0q", L.MatMulDesc)
 _QGEMM = _Packer("@3qiP2i2f3i2q", L.QGemmDesc)
+_GEMM_Q4 = _Packer("@3q2i2f2q", L.GemmQ4Desc)
+_KV_CACHE = _Packer("@q4i4P", L.KvCacheDesc)
+_KV_APPEND = _Packer("@q5i7q", L.KvAppendDesc)
+_ATTN_DECODE = _Packer("@q4if2q", L.AttnDecodeDesc)
+_ATTN_PREFILL = _Packer("@3q6if4q", L.AttnPrefillDesc)
 # the zero points that one byte can hold, for calls with a single one
 _ZERO_POINTS = np.arange(-128, 256, dtype=np.int32)
 _ZERO_POINTS_AT = _ZERO_POINTS.ctypes.data
@@ -86,6 +91,70 @@ def _key(name, label):
     if name is None:
         return None
     return ctypes.byref(L.WeightKey(name.encode(), (label or "").encode()))
+
+
+def _invalid(msg):
+    return L.OhipError(L.E_INVALID, msg)
+
+
+def _heads(t, name, dtype, device):
+    """Checks [tokens, heads, channels] of a 16-bit `dtype` on GPU `device`, heads next to each other;
+    the elements between tokens."""
+    if t.dtype != dtype or t.get_device() != device:
+        raise _invalid(f"{name}: {dtype} on GPU {device} is expected")
+    try:
+        rows, per_head, one = t.stride()
+    except ValueError:
+        raise _invalid(f"{name}: [tokens, heads, channels] is expected") from None
+    _, heads, dim = t.shape
+    if (one != 1 and dim > 1) or (per_head != dim and heads > 1):
+        raise _invalid(f"{name}: a token's heads are not next to each other")
+    return rows if t.shape[0] > 1 else heads * dim
+
+
+def _table(t, name, dtype, device, shape):
+    if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or t.shape != shape:
+        raise _invalid(f"{name}: a contiguous {dtype} array of {tuple(shape)} on GPU {device} is expected")
+    return t.data_ptr()
+
+
+class KvCache:
+    """A paged cache of keys and values in 4 bits (the layout is ohip_kv_cache's, include/ohip.h), in
+    caller-owned tensors: codes uint8 [pages, kv_heads, page, 4, head_dim / 32, 4] of the keys and
+    [pages, kv_heads, page / 16, 16, 16, head_dim / 32] of the values, and float16
+    [pages, kv_heads, page, head_dim / group, 2] scales and minima of each."""
+
+    def __init__(self, k_codes, v_codes, k_params, v_params):
+        torch = _torch()
+        if k_codes.dim() != 6 or k_params.dim() != 5 or 0 in k_params.shape:
+            raise _invalid("KvCache: codes or parameters of another rank, or empty")
+        pages, kv, page, _, words, _ = k_codes.shape
+        self.device, self.dim, groups = k_codes.get_device(), 32 * words, k_params.shape[3]
+        self.pages, self.page, self.kv_heads, self.group = pages, page, kv, self.dim // groups
+        want = (((pages, kv, page, 4, words, 4), torch.uint8), ((pages, kv, page // 16, 16, 16, words), torch.uint8),
+                ((pages, kv, page, groups, 2), torch.float16), ((pages, kv, page, groups, 2), torch.float16))
+        self.tensors = (k_codes, v_codes, k_params, v_params)
+        for t, (shape, dtype) in zip(self.tensors, want):
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.get_device() != self.device:
+                raise _invalid(f"KvCache: a contiguous {dtype} tensor of {shape} on one device is expected")
+        if page % 16 or self.group * groups != self.dim:
+            raise _invalid("KvCache: pages are a multiple of 16 tokens, groups divide the head")
+        self.desc = _KV_CACHE(pages, page, kv, self.dim, self.group, *(t.data_ptr() for t in self.tensors))
+
+    @staticmethod
+    def empty(pages, page, kv_heads, head_dim, group=64, device=0):
+        """A cache of zeros."""
+        torch = _torch()
+        at = torch.device("cuda", device)
+        params = (pages, kv_heads, page, head_dim // group, 2)
+        return KvCache(torch.zeros((pages, kv_heads, page, 4, head_dim // 32, 4), dtype=torch.uint8, device=at),
+                       torch.zeros((pages, kv_heads, page // 16, 16, 16, head_dim // 32), dtype=torch.uint8, device=at),
+                       torch.zeros(params, dtype=torch.float16, device=at),
+                       torch.zeros(params, dtype=torch.float16, device=at))
+
+    @property
+    def nbytes(self):
+        return sum(t.nbytes for t in self.tensors)
 
 
 class Weight:
@@ -234,6 +303,37 @@ class HipContext:
             None if sc is None else sc.ctypes.data_as(ctypes.c_void_p), 0 if sc is None else sc.size,
             ctypes.byref(h)))
         return Weight(self, h, "qconv", L.I8, w.shape, name is not None)
+
+    def weight_q4(self, codes, scales, zero_points=None, k=None, dtype=None, name=None, label="Gemm.B4"):
+        """A weight [K, N] of 4-bit codes (ohip_weight_q4): codes uint8 [N, blocks, group / 2], scales [N, blocks]
+        (float32 or float16, rounded to `dtype`, the activations' type, by default their own), zero_points uint8
+        [N, ceil(blocks / 2)] or None (8 everywhere); k if K does not fill the last block."""
+        codes, scales = np.ascontiguousarray(codes), np.asarray(scales)
+        if codes.ndim != 3 or codes.dtype != np.uint8 or scales.shape != codes.shape[:2]:
+            raise _invalid("weight_q4: codes uint8 [N, blocks, group / 2] and scales [N, blocks]")
+        n, blocks, half = codes.shape
+        k = blocks * 2 * half if k is None else k
+        if not blocks or not half or (k + 2 * half - 1) // (2 * half) != blocks:
+            raise _invalid("weight_q4: K does not end in the last block")
+        dtype = (L.F16 if scales.dtype == np.float16 else L.F32) if dtype is None else dtype
+        if dtype == L.F32:
+            scales = np.ascontiguousarray(scales, np.float32)
+        elif dtype == L.F16:
+            scales = np.ascontiguousarray(scales, np.float16)
+        elif dtype == L.BF16:
+            torch = _torch()
+            scales = torch.from_numpy(np.array(scales, np.float32)).to(torch.bfloat16).view(torch.int16).numpy()
+        else:
+            raise _invalid("weight_q4: dtype")
+        if zero_points is not None:
+            zero_points = np.ascontiguousarray(zero_points)
+            if zero_points.dtype != np.uint8 or zero_points.shape != (n, (blocks + 1) // 2):
+                raise _invalid("weight_q4: zero points uint8 [N, ceil(blocks / 2)]")
+        h = ctypes.c_void_p()
+        L.check(L.lib().ohip_weight_q4(self.h, _key(name, label), codes.ctypes.data, k, n, 2 * half, dtype,
+                                       scales.ctypes.data, None if zero_points is None else zero_points.ctypes.data,
+                                       ctypes.byref(h)))
+        return Weight(self, h, "q4", dtype, (k, n), name is not None)
 
     # --------------------------------------------------------------- ops
     def gemm(self, a, w, c=None, alpha=1.0, beta=1.0, trans_a=False, act=L.ACT_NONE, act_lo=0.0, act_hi=0.0,
@@ -401,4 +501,130 @@ class HipContext:
                         pads[0], pads[1], pads[2], pads[3], ohip_dtype(x.dtype), int(x_zp), out_kind, x_scale,
                         y_scale, y_zp, lo, hi, in_layout, out_layout)
         L.check(L.lib().ohip_qconv2d(self.h, ctypes.byref(d), _ptr(x), w.handle, _ptr(bias), _ptr(out)))
+        return out
+
+    # --------------------------------------------------------------- serving
+    def gemm_q4(self, a, w, bias=None, act=L.ACT_NONE, act_lo=0.0, act_hi=0.0, out=None):
+        """act(a @ w + bias) of a [M, K] and a weight of weight_q4 (ohip_gemm_q4); bias [N] of a's type."""
+        m, k = a.shape
+        n = w.shape[1]
+        if out is None:
+            out = _torch().empty((m, n), dtype=a.dtype, device=a.device)
+        at = self.device
+        if (a.get_device() != at or out.get_device() != at or out.dtype != a.dtype or out.shape != (m, n)
+                or (k > 1 and a.stride(1) != 1) or (n > 1 and out.stride(1) != 1)):
+            raise _invalid("gemm_q4: a [M, K] and out [M, N] of one type on the context's GPU, rows contiguous")
+        if bias is not None and (bias.dtype != a.dtype or bias.get_device() != at or not bias.is_contiguous()
+                                 or bias.numel() != n):
+            raise _invalid("gemm_q4: bias [N] of the activations' type")
+        d = _GEMM_Q4(m, k, n, ohip_dtype(a.dtype), act, act_lo, act_hi, a.stride(0) if m > 1 else k,
+                     out.stride(0) if m > 1 else n)
+        rc = L.raw("ohip_gemm_q4")(self.h, d, a.data_ptr(), w.handle, _ptr(bias), out.data_ptr())
+        if rc:
+            L.check(rc)
+        return out
+
+    def kv_cache(self, pages, page, kv_heads, head_dim, group=64):
+        """An empty KvCache on this context's GPU."""
+        return KvCache.empty(pages, page, kv_heads, head_dim, group, self.device)
+
+    def kv_append(self, cache, k, v, slots, q=None, positions=None, cos=None, sin=None, interleaved=False,
+                  out_held=True, q_out=None, k_out=None, v_out=None):
+        """Appends keys and values [tokens, kv_heads, dim] at `slots` (int32, page * page size + place; negative:
+        not written), keys and queries rotated by rows `positions` (int32) of cos / sin (float32 [positions,
+        rot / 2]); see ohip_kv_append.  Returns (q_out, k_out, v_out): the rotated queries, and keys and values
+        as the cache holds them (out_held) or as they went in; k_out / v_out False: not wanted."""
+        torch = _torch()
+        at, dt, f32, i32 = self.device, k.dtype, torch.float32, torch.int32
+        tokens, kv, dim = k.shape if k.dim() == 3 else (0, 0, 0)
+        if kv != cache.kv_heads or dim != cache.dim or v.shape != k.shape or cache.device != at:
+            raise _invalid("kv_append: keys and values [tokens, kv_heads, dim] of the cache")
+        ldk, ldv = _heads(k, "kv_append: k", dt, at), _heads(v, "kv_append: v", dt, at)
+        heads, ldq, ldqo, rot, rows = 0, 0, 0, 0, 0
+        if q is not None:
+            if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim:
+                raise _invalid("kv_append: q [tokens, heads, dim]")
+            heads, ldq = q.shape[1], _heads(q, "kv_append: q", dt, at)
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
+            elif q_out.shape != q.shape:
+                raise _invalid("kv_append: q_out has another shape than q")
+            ldqo = _heads(q_out, "kv_append: q_out", dt, at)
+        ld = []
+        outs = []
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is False:
+                ld.append(0)
+                outs.append(None)
+                continue
+            if t is None:
+                t = torch.empty(k.shape, dtype=dt, device=k.device)
+            elif t.shape != k.shape:
+                raise _invalid(f"kv_append: {name} has another shape than k")
+            ld.append(_heads(t, name, dt, at))
+            outs.append(t)
+        pos = cs = sn = None
+        if cos is not None:
+            rows, rot = cos.shape[0], 2 * cos.shape[1]
+            cs = _table(cos, "kv_append: cos", f32, at, cos.shape)
+            sn = _table(sin, "kv_append: sin", f32, at, cos.shape)
+            pos = _table(positions, "kv_append: positions", i32, at, (tokens,))
+        d = _KV_APPEND(tokens, ohip_dtype(dt), heads, rot, int(interleaved), int(out_held), rows, ldq, ldk, ldv, ldqo,
+                       ld[0], ld[1])
+        rc = L.raw("ohip_kv_append")(self.h, d, cache.desc, _ptr(q), k.data_ptr(), v.data_ptr(), pos, cs, sn,
+                                     _table(slots, "kv_append: slots", i32, at, (tokens,)), _ptr(q_out),
+                                     _ptr(outs[0]), _ptr(outs[1]))
+        if rc:
+            L.check(rc)
+        return q_out, outs[0], outs[1]
+
+    def attn_decode(self, q, cache, table, lens, scale=None, window=0, out=None):
+        """Attention of one query token a sequence [batch, heads, dim] over the first lens[b] (int32) tokens of
+        the pages table[b] (int32 [batch, entries]) of `cache`, at most the last `window` of them (0: all);
+        scale: 1 / sqrt(dim) by default (ohip_attn_decode)."""
+        at, dt = self.device, q.dtype
+        ldq = _heads(q, "attn_decode: q", dt, at)
+        batch, heads, dim = q.shape
+        if dim != cache.dim or cache.device != at:
+            raise _invalid("attn_decode: q [batch, heads, dim] of the cache")
+        if out is None:
+            out = _torch().empty(q.shape, dtype=dt, device=q.device)
+        elif out.shape != q.shape:
+            raise _invalid("attn_decode: out has another shape than q")
+        i32 = _TORCH_DT[L.I32]
+        width = table.shape[-1]
+        d = _ATTN_DECODE(batch, ohip_dtype(dt), heads, width, window, dim ** -0.5 if scale is None else scale, ldq,
+                         _heads(out, "attn_decode: out", dt, at))
+        rc = L.raw("ohip_attn_decode")(self.h, d, cache.desc, q.data_ptr(),
+                                       _table(table, "attn_decode: table", i32, at, (batch, width)),
+                                       _table(lens, "attn_decode: lens", i32, at, (batch,)), out.data_ptr())
+        if rc:
+            L.check(rc)
+        return out
+
+    def attn_prefill(self, q, k, v, cu_q, cu_k=None, scale=None, causal=True, window=0, out=None):
+        """Attention over packed sequences: q [tokens, heads, dim], k and v [key tokens, kv_heads, dim], int32
+        offsets cu_q (and cu_k, by default the same) of sequences + 1 entries; see ohip_attn_prefill."""
+        at, dt = self.device, q.dtype
+        ldq, ldk, ldv = (_heads(t, n, dt, at) for t, n in ((q, "attn_prefill: q"), (k, "attn_prefill: k"),
+                                                           (v, "attn_prefill: v")))
+        (tokens, heads, dim), (keys, kv, kdim) = q.shape, k.shape
+        if v.shape != k.shape or kdim != dim:
+            raise _invalid("attn_prefill: k and v [key tokens, kv_heads, dim], dim as q")
+        if out is None:
+            out = _torch().empty(q.shape, dtype=dt, device=q.device)
+        elif out.shape != q.shape:
+            raise _invalid("attn_prefill: out has another shape than q")
+        cu_k = cu_q if cu_k is None else cu_k
+        i32, seqs = _TORCH_DT[L.I32], cu_q.shape[0] - 1
+        if seqs < 0:
+            raise _invalid("attn_prefill: cu_q needs an entry")
+        d = _ATTN_PREFILL(tokens, keys, seqs, ohip_dtype(dt), heads, kv, dim, int(causal), window,
+                          dim ** -0.5 if scale is None else scale, ldq, ldk, ldv,
+                          _heads(out, "attn_prefill: out", dt, at))
+        rc = L.raw("ohip_attn_prefill")(self.h, d, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                        _table(cu_q, "attn_prefill: cu_q", i32, at, (seqs + 1,)),
+                                        _table(cu_k, "attn_prefill: cu_k", i32, at, (seqs + 1,)), out.data_ptr())
+        if rc:
+            L.check(rc)
         return out
