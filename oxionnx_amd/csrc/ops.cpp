@@ -2560,6 +2560,8 @@ extern "C" int ohip_attn_prefill(ohip_ctx* ctx, const ohip_attn_prefill_desc* d,
   if ((rc = rows_check(q, p.ldq, wq, d->q_tokens, kWhere, "q")) || (rc = rows_check(k, p.ldk, wk, d->k_tokens, kWhere, "k")) ||
       (rc = rows_check(v, p.ldv, wk, d->k_tokens, kWhere, "v")) || (rc = rows_check(out, p.ldo, wq, d->q_tokens, kWhere, "out")))
     return rc;
+  // the kernel's loads address a tile of keys with 32 bits
+  if (p.ldk > (1 << 22) || p.ldv > (1 << 22)) return fail(OHIP_DECLINED, "ohip_attn_prefill: rows too far apart");
   p.cu_q = cu_q; p.cu_k = cu_k; p.q_tokens = d->q_tokens; p.k_tokens = d->k_tokens;
   p.seqs = (int)d->seqs; p.kv = d->kv_heads; p.g = d->heads / d->kv_heads; p.dim = d->head_dim;
   p.causal = d->causal != 0; p.window = d->window; p.c = d->scale * 1.4426950408889634f;

@@ -121,4 +121,31 @@ template <class T> __device__ __forceinline__ constexpr float code_bias(int elem
   return std::is_same<T, _Float16>::value ? ((element & 2) ? 64.0f : 1024.0f) : 128.0f;
 }
 
+// the larger of a value and the other half wave's
+__device__ __forceinline__ float max_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = r[0], b = r[1];
+  return __builtin_fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float sum_halves(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = r[0], b = r[1];
+  return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// A barrier that publishes LDS stores; global loads may stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A buffer resource of `bytes` from a wave-uniform address: loads beyond read as zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_resource(const char* at, int bytes) {
+  const uint64_t a = (uint64_t)at;
+  const uint64_t u = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) << 32;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
 }  // namespace ohip
