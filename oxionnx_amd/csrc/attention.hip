@@ -3,21 +3,20 @@
 
 namespace ohip {
 
-// A block has BQ = 32 * NW * QB query rows of one head, QB blocks of 32 a wave,
-// and walks the keys they see in tiles of 64 that all its waves share through
-// LDS.  S^T = K Q^T, so a lane holds one query (its column) and the softmax's
-// running maximum and sum need one exchange between a lane and the one 32
-// further; O^T = V^T P^T takes P as it lies in the registers: k index 8 h + j
-// (h = lane / 32) stands for key 4 h + j of a block of 8, then of the next,
-// and V's fragments come from LDS through the transposing read.
+// A block has 32 * NW query rows of one head, 32 a wave, and walks the keys
+// they see in tiles of 64 that all its waves share through LDS.  S^T = K Q^T,
+// so a lane holds one query (its column) and the softmax's running maximum and
+// sum need one exchange between a lane and the one 32 further; O^T = V^T P^T
+// takes P as it lies in the registers: k index 8 h + j (h = lane / 32) stands
+// for key 4 h + j of a block of 8, then of the next, and V's fragments come
+// from LDS through the transposing read.
 //
-// LDS: two buffers of a K and a V tile.  Each thread loads its part of tile
-// t + 1 into registers before the products of tile t and stores it to LDS
-// after them, so one barrier a tile is enough.  (Loads that write LDS directly
-// save the registers, but the compiler waits for all of them before any
-// transposing read.)  Rows past the sequence's end and channels past the head
-// read as zeros (the buffer's range check).
-constexpr int kPrefillK = 64;
+// Bound: the matrix products, with about as many cycles of vector instructions
+// (two thirds of them the exponentials and their arguments), so each stage
+// interleaves the softmax of one half tile with the products of its
+// neighbours; and the latency of the tiles, which are loaded straight into
+// LDS three passes ahead.
+constexpr int kPrefillK = 64, kPrefillBufs = 4;
 
 // Slot of 16-byte chunk c of a staged row r: rows of 16 (8) chunks, XOR with a
 // permutation of r's low bits that puts 16 consecutive rows of one chunk (the
@@ -41,20 +40,24 @@ __device__ __forceinline__ int slot_sequence(const int32_t* cu, int seqs, int64_
     const int64_t c = i < seqs ? min(max((int64_t)cu[i], (int64_t)0), total) : 0;
     n += __popcll(__ballot(i < seqs && c / bq + i <= tile));
   }
-  return n - 1;
+  return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-template <class T, int D, int NW, int QB>
-__global__ void __launch_bounds__(64 * NW, QB == 1 ? 2 : 1)
+template <class T, int D, int NW>
+__global__ void __launch_bounds__(64 * NW, 2)
 attn_prefill_kernel(const AttnPrefillArgs p) {
-  constexpr int BQ = 32 * NW * QB, BK = kPrefillK, KS = D / 16, OT = D / 32;
+  constexpr int BQ = 32 * NW, BK = kPrefillK, KS = D / 16, OT = D / 32;
   constexpr int CH = D > 64 ? 16 : 8, RB = CH * 16;     // chunks and bytes of a staged row
   constexpr int NL = BK * CH / (64 * NW);               // loads a thread of a tile
+  constexpr int NB = kPrefillBufs;
   constexpr int kTile = BK * RB;
   static_assert(NL >= 1 && (64 / CH) * NW % 16 == 0, "a thread's loads share their swizzle");
-  __shared__ __align__(16) char lds[2][2][kTile];       // [buffer][K, V]
+  // K and V tiles, each a variable of its own: the compiler then knows which
+  // loads a fragment read may depend on, and waits for no later ones
+  __shared__ __align__(256) char lk0[kTile], lk1[kTile], lk2[kTile], lk3[kTile];
+  __shared__ __align__(256) char lv0[kTile], lv1[kTile], lv2[kTile], lv3[kTile];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, h2 = lane >> 5;
   // heads of one key head next to each other in time, key heads eight apart: an XCD's L2 holds its own
@@ -75,33 +78,29 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
   int kend = nk, kbeg = 0;
   if (p.causal) kend = min(nk, max(0, qt + qrows + shift));
   if (p.window > 0) kbeg = max(0, qt + shift - p.window + 1) / BK * BK;
-  // this wave's queries qw .. qw + 32 QB - 1; its lanes' are qw + 32 b + r
-  const int qw = qt + wave * 32 * QB;
-  const int wend = p.causal ? min(nk, min(qw + 32 * QB, nq) + shift) : nk;   // keys that any of them sees
-  const bool idle = qw >= nq;
+  const int tiles = kend > kbeg ? (kend - kbeg + BK - 1) / BK : 0;
+  const int qw = __builtin_amdgcn_readfirstlane(qt + wave * 32);   // this wave's first query; its lanes' are qw + r
+  // half tiles that this wave's queries see
+  const int wend = min(kend, p.causal ? min(qw + 32, nq) + shift : nk);
+  const int halves = qw < nq && wend > kbeg ? (wend - kbeg + 31) / 32 : 0;
 
-  u32x4 qf[QB][KS];
-#pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    const T* src = static_cast<const T*>(p.q) + (q0 + min(qw + 32 * b + r, nq - 1)) * p.ldq + (int64_t)head * p.dim;
+  u32x4 qf[KS];
+  {
+    const T* src = static_cast<const T*>(p.q) + (q0 + min(qw + r, nq - 1)) * p.ldq + (int64_t)head * p.dim;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int ch = 16 * s + 8 * h2;
-      qf[b][s] = u32x4{0, 0, 0, 0};
-      if (ch < p.dim) __builtin_memcpy(&qf[b][s], __builtin_assume_aligned(src + ch, 16), 16);
+      qf[s] = u32x4{0, 0, 0, 0};
+      if (ch < p.dim) __builtin_memcpy(&qf[s], __builtin_assume_aligned(src + ch, 16), 16);
     }
   }
-  f32x16 o[QB][OT];
-  float mx[QB], l[QB];
+  f32x16 o[OT];
 #pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    mx[b] = -__builtin_inff();
-    l[b] = 0.0f;
+  for (int t = 0; t < OT; ++t)
 #pragma unroll
-    for (int t = 0; t < OT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[b][t][i] = 0.0f;
-  }
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
+  float base = -__builtin_inff(), l = 0.0f;   // the maximum that weights are taken against, times c; their sum
+
   const char* kb = static_cast<const char*>(p.k) + (k0 * p.ldk + (int64_t)kvh * p.dim) * 2;
   const char* vb = static_cast<const char*>(p.v) + (k0 * p.ldv + (int64_t)kvh * p.dim) * 2;
   // this thread's loads: row (i * NW + wave) * (64 / CH) + lane / CH, slot lane % CH
@@ -111,145 +110,270 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
   const int kvoff = inside ? (int)(lrow * p.ldk * 2) + chunk * 16 : (int)0x80000000u;
   const int vvoff = inside ? (int)(lrow * p.ldv * 2) + chunk * 16 : (int)0x80000000u;
   const int kstep = (int)(NW * (64 / CH) * p.ldk * 2), vstep = (int)(NW * (64 / CH) * p.ldv * 2);
-  u32x4 kin[NL], vin[NL];
-  auto fetch = [&](int kt) __attribute__((always_inline)) {
-    const int rows = min(nk - kt, BK);   // > 0: rows of the sequence from kt on
-    const auto kr = rows_resource(kb + (int64_t)kt * p.ldk * 2, (int)((rows - 1) * p.ldk + p.dim) * 2);
-    const auto vr = rows_resource(vb + (int64_t)kt * p.ldv * 2, (int)((rows - 1) * p.ldv + p.dim) * 2);
+  // tile t into `to`; a tile past the end reads as zeros (every pass issues
+  // the same number of loads, which its waits count)
+  auto load = [&](const char* at, int64_t ld, int t, int voff, int step, char* to) __attribute__((always_inline)) {
+    const int kt = kbeg + t * BK, rows = max(0, min(nk - kt, BK));
+    const auto rs = rows_resource(at + (int64_t)min(kt, nk) * ld * 2, max(0, (int)((rows - 1) * ld + p.dim) * 2));
 #pragma unroll
-    for (int i = 0; i < NL; ++i) kin[i] = __builtin_amdgcn_raw_buffer_load_b128(kr, kvoff + i * kstep, 0, 0);
-#pragma unroll
-    for (int i = 0; i < NL; ++i) vin[i] = __builtin_amdgcn_raw_buffer_load_b128(vr, vvoff + i * vstep, 0, 0);
+    for (int i = 0; i < NL; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + (i * NW + wave) * 1024), 16,
+                                               voff + i * step, 0, 0, 0);
   };
-  char* const mine = lds[0][0] + threadIdx.x * 16;
-  auto put = [&](int buf) __attribute__((always_inline)) {
+  // Fragment addresses within a tile: rows are aligned to their swizzle, so a
+  // chunk is an XOR.  K: row r, chunk 2 s + h2.  V: keys 8 j + 4 h2 +
+  // (lane % 16) / 4 on, channels 16 ((lane / 16) % 2) + 4 (lane % 4) of the 32
+  // from 32 t on.
+  int ka[KS], va[2][OT];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4*>(mine + buf * 2 * kTile + i * NW * 1024) = kin[i];
+  for (int k = 0; k < KS; ++k) ka[k] = (r * RB + ((h2 ^ row_swizzle<CH>(r)) * 16)) ^ (32 * k);
 #pragma unroll
-    for (int i = 0; i < NL; ++i) *reinterpret_cast<u32x4*>(mine + (buf * 2 + 1) * kTile + i * NW * 1024) = vin[i];
-  };
-  // fragment addresses: K row r chunk 2 s + h2; V keys 4 h2 + (lane % 16) / 4 on, channels 16 ((lane / 16) % 2) + 4 (lane % 4)
-  const int ksw = row_swizzle<CH>(r);
-  const int vrow = 4 * h2 + (lane & 15) / 4, vch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vby = 8 * (lane & 1);
+  for (int j = 0; j < 2; ++j) {
+    const int row = 8 * j + 4 * h2 + (lane & 15) / 4;
+    const int at = row * RB + (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ row_swizzle<CH>(row)) * 16) + 8 * (lane & 1);
+#pragma unroll
+    for (int t = 0; t < OT; ++t) va[j][t] = at ^ (64 * t);
+  }
 
-  auto tile_pass = [&](int kt, int buf) __attribute__((always_inline)) {
-    const char* ks = lds[buf][0];
-    const char* vs = lds[buf][1];
-    f32x16 s[QB][2];
+  // The three steps of a half tile of 32 keys.  Each stage of the pipeline
+  // runs one half's softmax between the next one's scores and the previous
+  // one's values, so that the matrix unit has independent work under the
+  // softmax's vector instructions (in one wave: the waves of a SIMD pass the
+  // barriers together and would all be at the same step).
+  auto key_frag = [&](const char* at, int k) __attribute__((always_inline)) -> u32x4 {
+    return *reinterpret_cast<const u32x4*>(at + ka[k]);
+  };
+  auto value_frag = [&](const char* at, int k, int t) __attribute__((always_inline)) -> u32x4 {   // 16 keys from 16 k on
+    u32x4 f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int j = 0; j < 2; ++j) {
+      const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(at + va[j][t] + 16 * k * RB));
+      const u32x2 w = __builtin_bit_cast(u32x2, v);
+      f[2 * j] = w.x;
+      f[2 * j + 1] = w.y;
+    }
+    return f;
+  };
+  auto scores = [&](const char* at, f32x16& s) __attribute__((always_inline)) {
 #pragma unroll
-      for (int b = 0; b < QB; ++b)
+    for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][t][i] = 0.0f;
+    for (int k = 0; k < KS; ++k) s = mma32<T>(key_frag(at, k), qf[k], s);
+  };
+  auto values = [&](const char* at, const u32x4 (&pf)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const u32x4 f = *reinterpret_cast<const u32x4*>(ks + (32 * t + r) * RB + (((2 * k + h2) ^ ksw) * 16));
+    for (int i = 0; i < 2 * OT; ++i) o[i % OT] = mma32<T>(value_frag(at, i / OT, i % OT), pf[i / OT], o[i % OT]);
+  };
+  // weights of half j from its scores, against a maximum that is taken anew
+  // only when a score exceeds it by more than 8 powers of two; returns what
+  // the sums so far have to be multiplied with
+  auto mask = [&](int j, f32x16& s) __attribute__((always_inline)) {
+    const int kj = kbeg + 32 * j;
+    if (kj + 32 > nk || (p.causal && kj + 31 > qw + shift) || (p.window > 0 && kj <= qw + 31 + shift - p.window)) {
+      const int last = (p.causal ? min(nk - 1, qw + r + shift) : nk - 1) - kj - 4 * h2;
+      const int low = (p.window > 0 ? qw + r + shift - p.window : -1) - kj - 4 * h2;
 #pragma unroll
-        for (int b = 0; b < QB; ++b) s[b][t] = mma32<T>(f, qf[b][k], s[b][t]);
+      for (int i = 0; i < 16; ++i) {
+        const int key = 8 * (i / 4) + i % 4;
+        if (key > last || key <= low) s[i] = -__builtin_inff();
       }
     }
-    u32x4 pf[QB][4];
+  };
+  // the sums so far wait for a factor
+  int grown = 0;
+  float keep = 1.0f;
+  auto softmax = [&](f32x16& s, u32x4 (&pf)[2]) __attribute__((always_inline)) {
+    float m = s[0];
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-      const int qi = qw + 32 * b;   // the block's first query
-      if (kt + BK > nk || (p.causal && kt + BK - 1 > qi + shift) || (p.window > 0 && kt <= qi + 31 + shift - p.window)) {
-        const int last = p.causal ? min(nk - 1, qi + r + shift) : nk - 1;
-        const int low = p.window > 0 ? qi + r + shift - p.window : -1;
+    for (int i = 1; i < 16; ++i) m = __builtin_fmaxf(m, s[i]);
+    m = max_halves(m) * p.c;
+    const bool grow = __any(m - base > 8.0f);
+    const float now = grow ? __builtin_fmaxf(base, m) : base;
+    const float off = now == -__builtin_inff() ? 0.0f : now;
+    keep = __builtin_amdgcn_exp2f(base - off);   // 0 the first time
+    base = now;
+    l *= grow ? keep : 1.0f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = kt + 32 * t + 8 * (i / 4) + 4 * h2 + i % 4;
-            if (key > last || key <= low) s[b][t][i] = -__builtin_inff();
-          }
-      }
-      float m = s[b][0][0];
-#pragma unroll
-      for (int i = 1; i < 32; ++i) m = __builtin_fmaxf(m, s[b][i / 16][i % 16]);
-      m = max_halves(m);
-      if (__any(m > mx[b])) {
-        const float now = __builtin_fmaxf(mx[b], m);
-        const float keep = now == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((mx[b] - now) * p.c);
-        mx[b] = now;
-        l[b] *= keep;
-#pragma unroll
-        for (int t = 0; t < OT; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[b][t][i] *= keep;
-      }
-      const float base = mx[b] == -__builtin_inff() ? 0.0f : mx[b] * p.c;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[b][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][t][i], p.c, -base));
-          l[b] += s[b][t][i];
-        }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          pf[b][k][j] = pack2<T>(s[b][k / 2][8 * (k % 2) + 2 * j], s[b][k / 2][8 * (k % 2) + 2 * j + 1]);
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], p.c, -off));
+      l += s[i];
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k)   // 16 keys
+    for (int i = 0; i < 8; ++i) pf[i / 4][i % 4] = pack2<T>(s[2 * i], s[2 * i + 1]);
+    grown = __builtin_amdgcn_readfirstlane((int)grow);
+    asm("" : "+s"(grown));   // not known to be `grow`: the branch on it stays in the next stage
+  };
+  auto rescale = [&]() __attribute__((always_inline)) {
+    if (grown)
 #pragma unroll
-      for (int t = 0; t < OT; ++t) {
-        u32x4 f;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = 16 * k + 8 * j + vrow;
-          const char* at = vs + row * RB + (((4 * t + vch) ^ row_swizzle<CH>(row)) * 16) + vby;
-          const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
-          const u32x2 w = __builtin_bit_cast(u32x2, v);
-          f[2 * j] = w.x;
-          f[2 * j + 1] = w.y;
-        }
-#pragma unroll
-        for (int b = 0; b < QB; ++b) o[b][t] = mma32<T>(f, pf[b][k], o[b][t]);
-      }
+      for (int i = 0; i < 16 * OT; ++i) o[i / 16][i % 16] *= keep;
   };
 
-  if (kbeg < kend) {
-    fetch(kbeg);
-    put(0);
-  }
-  int buf = 0;
-  for (int kt = kbeg; kt < kend; kt += BK, buf ^= 1) {
-    const bool more = kt + BK < kend;
-    lds_barrier();
-    if (more) fetch(kt + BK);
-    if (!idle && kt < wend) tile_pass(kt, buf);
-    if (more) put(buf ^ 1);   // last read in the pass before this one
-  }
+  f32x16 s[2];
+  u32x4 pf[2];
+  // stage of half j: scores of half j + 1 from LDS at kn, softmax of half j,
+  // values of half j - 1 at vn
+  auto stage = [&](int j, const char* kn, const char* vn, f32x16& cur, f32x16& next) __attribute__((always_inline)) {
+    u32x4 w[2];
+    rescale();
+    mask(j, cur);
+    u32x4 vf[2 * OT], kf[KS];
 #pragma unroll
-  for (int b = 0; b < QB; ++b) {
-    const int qi = qw + 32 * b + r;
-    const float sum = sum_halves(l[b]);
-    if (qi >= nq) continue;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // a row that sees no key: zeros
-    T* dst = static_cast<T*>(p.out) + (q0 + qi) * p.ldo + (int64_t)head * p.dim;
+    for (int i = 0; i < 2 * OT; ++i) {
+      vf[i] = value_frag(vn, i / OT, i % OT);
+      kf[i] = key_frag(kn, i);
+    }
 #pragma unroll
-    for (int t = 0; t < OT; ++t)
+    for (int i = 0; i < 16; ++i) next[i] = 0.0f;
+    static_assert(KS == 2 * OT, "one of each in turn: the scores' products wait for each other");
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ch = 32 * t + 8 * i + 4 * h2;
-        const u32x2 w = {pack2<T>(o[b][t][4 * i] * inv, o[b][t][4 * i + 1] * inv),
-                         pack2<T>(o[b][t][4 * i + 2] * inv, o[b][t][4 * i + 3] * inv)};
-        if (ch < p.dim) *reinterpret_cast<u32x2*>(dst + ch) = w;
-      }
+    for (int i = 0; i < KS; ++i) {
+      o[i % OT] = mma32<T>(vf[i], pf[i / OT], o[i % OT]);
+      next = mma32<T>(kf[i], qf[i], next);
+    }
+    softmax(cur, w);
+    // In the wave's order: the fragments' loads and the maximum between the
+    // first products, then the exponentials (530 us for the 8192-token prompt;
+    // 546 in the compiler's order, 562 with all loads in front).
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);     // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x402, 5, 0);     // vector instructions
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);       // a matrix product
+    }
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 7, 0);
+    }
+    // here, not sunk past the next stage's branches
+    asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(l));
+    pf[0] = w[0];
+    pf[1] = w[1];
+  };
+  constexpr int kHalf = 32 * RB;
+  // Pass t: scores of tile t + 1, values of tile t.  All waves go through the
+  // block's passes; a wave computes while its queries see keys.  K tile i is
+  // in variable i % NB and so is V tile i: pass t may overwrite K tile t and V
+  // tile t - 1, the last ones that pass t - 1 read, with tiles t + NB and
+  // t + NB - 1, which have NB - 1 passes to arrive.
+  auto kvar = [&](auto i) __attribute__((always_inline)) -> char* {
+    constexpr int v = decltype(i)::value % NB;
+    if constexpr (v == 0) return lk0; else if constexpr (v == 1) return lk1; else if constexpr (v == 2) return lk2; else return lk3;
+  };
+  auto vvar = [&](auto i) __attribute__((always_inline)) -> char* {
+    constexpr int v = decltype(i)::value % NB;
+    if constexpr (v == 0) return lv0; else if constexpr (v == 1) return lv1; else if constexpr (v == 2) return lv2; else return lv3;
+  };
+  int t = 0;
+  auto begin = [&](auto at) __attribute__((always_inline)) {   // at: t % NB
+    constexpr int m = decltype(at)::value;
+    loads_barrier<(NB - 2) * 2 * NL>();   // all but those of the last NB - 2 passes
+    load(kb, p.ldk, t + NB, kvoff, kstep, kvar(std::integral_constant<int, m>()));
+    load(vb, p.ldv, t + NB - 1, vvoff, vstep, vvar(std::integral_constant<int, m + NB - 1>()));
+  };
+  auto pass = [&](auto at) __attribute__((always_inline)) {
+    constexpr int m = decltype(at)::value;
+    const char* kn = kvar(std::integral_constant<int, m + 1>());
+    const char* vn = vvar(std::integral_constant<int, m>());
+    begin(at);
+    stage(2 * t + 1, kn, vn, s[1], s[0]);
+    stage(2 * t + 2, kn + kHalf, vn + kHalf, s[0], s[1]);
+    ++t;
+  };
+  auto last = [&](auto at) __attribute__((always_inline)) {   // the last one or two halves' values
+    const char* vn = vvar(at);
+    begin(at);
+    rescale();
+    values(vn, pf);
+    if (2 * t + 1 < halves) {
+      mask(2 * t + 1, s[1]);
+      softmax(s[1], pf);
+      rescale();
+      values(vn + kHalf, pf);
+    }
+    ++t;
+  };
+  using C0 = std::integral_constant<int, 0>;
+  using C1 = std::integral_constant<int, 1>;
+  using C2 = std::integral_constant<int, 2>;
+  using C3 = std::integral_constant<int, 3>;
+  if (tiles) {
+    load(kb, p.ldk, 0, kvoff, kstep, lk0);
+    load(vb, p.ldv, 0, vvoff, vstep, lv0);
+    load(kb, p.ldk, 1, kvoff, kstep, lk1);
+    load(vb, p.ldv, 1, vvoff, vstep, lv1);
+    load(kb, p.ldk, 2, kvoff, kstep, lk2);
+    load(vb, p.ldv, 2, vvoff, vstep, lv2);
+    load(kb, p.ldk, 3, kvoff, kstep, lk3);
+    loads_barrier<6 * NL>();   // K tile 0
+    if (halves > 0) {
+      scores(lk0, s[0]);
+      mask(0, s[0]);
+      scores(lk0 + kHalf, s[1]);
+      softmax(s[0], pf);
+    }
   }
+  while (2 * t + 8 < halves) {
+    pass(C0());
+    pass(C1());
+    pass(C2());
+    pass(C3());
+  }
+  if (2 * t + 2 < halves) {
+    pass(C0());
+    if (2 * t + 2 < halves) {
+      pass(C1());
+      if (2 * t + 2 < halves) pass(C2());
+    }
+  }
+  if (halves > 0) {
+    switch (t % NB) {
+      case 0: last(C0()); break;
+      case 1: last(C1()); break;
+      case 2: last(C2()); break;
+      default: last(C3()); break;
+    }
+  }
+  while (t < tiles) {
+    switch (t % NB) {
+      case 0: begin(C0()); break;
+      case 1: begin(C1()); break;
+      case 2: begin(C2()); break;
+      default: begin(C3()); break;
+    }
+    ++t;
+  }
+  loads_barrier<0>();   // those of tiles past the end write LDS too
+
+  const int qi = qw + r;
+  const float sum = sum_halves(l);
+  if (qi >= nq) return;
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // a row that sees no key: zeros
+  T* dst = static_cast<T*>(p.out) + (q0 + qi) * p.ldo + (int64_t)head * p.dim;
+#pragma unroll
+  for (int t = 0; t < OT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ch = 32 * t + 8 * i + 4 * h2;
+      const u32x2 w = {pack2<T>(o[t][4 * i] * inv, o[t][4 * i + 1] * inv), pack2<T>(o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv)};
+      if (ch < p.dim) *reinterpret_cast<u32x2*>(dst + ch) = w;
+    }
 }
 
-template <class T, int D, int NW, int QB> static hipError_t prefill_l(const AttnPrefillArgs& p, hipStream_t st) {
-  constexpr int BQ = 32 * NW * QB;
-  hipLaunchKernelGGL((attn_prefill_kernel<T, D, NW, QB>), dim3((unsigned)(p.kv * p.g), (unsigned)(p.q_tokens / BQ + p.seqs)),
+template <class T, int D, int NW> static hipError_t prefill_l(const AttnPrefillArgs& p, hipStream_t st) {
+  constexpr int BQ = 32 * NW;
+  hipLaunchKernelGGL((attn_prefill_kernel<T, D, NW>), dim3((unsigned)(p.kv * p.g), (unsigned)(p.q_tokens / BQ + p.seqs)),
                      dim3(64 * NW), 0, st, p);
   return hipGetLastError();
 }
 template <class T, int D> static hipError_t prefill_d(const AttnPrefillArgs& p, hipStream_t st) {
-  return prefill_l<T, D, 8, 1>(p, st);
+  // Eight waves (256 queries) share each tile of keys; where that leaves CUs
+  // without a block, four: 1000 queries x 32 heads of 3000-4000 keys 58 us
+  // against 71, 8192 x 32 728 against 530.
+  const int64_t wide = (int64_t)p.kv * p.g * (p.q_tokens / 256 + p.seqs);
+  return wide < 256 ? prefill_l<T, D, 4>(p, st) : prefill_l<T, D, 8>(p, st);
 }
 template <class T> static hipError_t prefill_t(const AttnPrefillArgs& p, hipStream_t st) {
   if (p.dim <= 64) return prefill_d<T, 64>(p, st);

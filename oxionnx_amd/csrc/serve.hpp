@@ -133,11 +133,17 @@ __device__ __forceinline__ float sum_halves(float v) {
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
 
-// A barrier that publishes LDS stores; global loads may stay in flight.
-__device__ __forceinline__ void lds_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+// Waits for all but the wave's last N loads and for its LDS reads, then the
+// block's barrier: the loads that write LDS are there for every wave, and what
+// the waves have read may be overwritten.  (A fence would wait for all loads.)
+template <int N> __device__ __forceinline__ void loads_barrier() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4));   // vmcnt(N) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // A buffer resource of `bytes` from a wave-uniform address: loads beyond read as zeros.
