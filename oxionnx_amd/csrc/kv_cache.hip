@@ -161,31 +161,73 @@ hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t 
 // The weights are split in two bf16 parts (16 bits together, f32's range: no
 // scale of the values can make them underflow).
 //
-// A block has the up to 16 query heads of one key head; its waves take steps
-// of 32 tokens.  S^T = K Q^T, lane l = 16 q + h: head h, tokens 4 q + r of
-// two tiles of 16, which is how O^T = V^T P^T wants its right operand when
-// the values' tokens are counted 4 q + j of the first tile, then of the
-// second.
+// A block has the up to 16 query heads of one key head and one range of the
+// sequence; its waves take steps of 32 tokens, the next step's codes in flight
+// under the present one's sums (three steps ahead cost registers and gained
+// nothing) and page entries 32 steps ahead.  A
+// step's scales and minima are loaded once, a word or more a lane, and spread
+// to the lanes that need them through LDS.  S^T = K Q^T,
+// lane l = 16 q + h: head h, tokens 4 q + r of two tiles of 16, which is how
+// O^T = V^T P^T wants its right operand when the values' tokens are counted
+// 4 q + j of the first tile, then of the second.
+//
+// Ranges of one sequence leave their maxima, sums and weighted values in `part`;
+// a second launch adds them in order.  (Counting the blocks and letting the
+// last one add saves the launch, but its fences write back and invalidate an
+// XCD's cache once a block: 355 us for a batch of 64, 76 with
+// the launch.)
 constexpr int kDecodeWaves = 4;
 
+// A sequence's tokens [lo, len), its steps of 32 tokens and their ranges.
+struct Span { int len, lo, begin, steps, ranges; };
+__device__ __forceinline__ Span span_of(const AttnDecodeArgs& p, int b) {
+  Span s;
+  s.len = (int)max((int64_t)0, min((int64_t)p.lens[b], (int64_t)p.width * p.tpp * 16));
+  s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
+  s.begin = s.lo / 32;
+  s.steps = (s.len + 31) / 32 - s.begin;
+  s.ranges = max(1, (s.steps + p.chunk - 1) / p.chunk);
+  return s;
+}
+
 template <class T, int D, int NG>
-__global__ void __launch_bounds__(64 * kDecodeWaves)
+__global__ void __launch_bounds__(64 * kDecodeWaves, NG == 4 ? 1 : 2)
 attn_decode_kernel(const AttnDecodeArgs p) {
+  constexpr int NW = kDecodeWaves;
   constexpr int KW = D / 32;   // steps of 32 channels
   constexpr int CI = D / 16;   // channels of a value column
   constexpr int SG = KW / NG;  // steps a group
   constexpr int RS = D + 4;
-  __shared__ float red[kDecodeWaves][16][RS];
-  __shared__ float red_m[kDecodeWaves][16], red_l[kDecodeWaves][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ float red[NW][16][RS];
+  __shared__ float red_m[NW][16], red_l[NW][16];
+  // of a wave's step, [token][group]: the keys' pairs, the values' scales and middles (of code 8)
+  __shared__ __align__(16) uint32_t spread_k[NW][32 * NG];
+  __shared__ __align__(16) float spread_v[NW][2][32 * NG];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int b = blockIdx.y, kvh = blockIdx.x % p.kv, hb = blockIdx.x / p.kv;
   const int nh = min(16, p.g - hb * 16);   // query heads of this block
   const int head0 = kvh * p.g + hb * 16;
-  const int64_t room = (int64_t)p.width * p.tpp * 16;
-  const int len = (int)max((int64_t)0, min((int64_t)p.lens[b], room));
-  const int lo = p.window > 0 ? max(0, len - p.window) : 0;
+  const Span span = span_of(p, b);
+  const int len = span.len, lo = span.lo, ranges = span.ranges, range = blockIdx.z;
+  if (range >= ranges) return;
+  // this block's range: steps of 32 tokens from `first` on
+  const int first = span.begin + range * p.chunk, steps = min(p.chunk, span.steps - range * p.chunk);
+  const int mine = steps > wave ? (steps - wave + NW - 1) / NW : 0;   // this wave's: first + wave + NW i
   const int32_t* table = p.table + (int64_t)b * p.width;
+  const int last_tile = len > 0 ? (len - 1) / 16 : 0;
+
+  // page and place within it of the wave's tiles: lane 2 i + t holds tile t of step i0 + i
+  auto entries = [&](int i0, int& id, int& place) __attribute__((always_inline)) {
+    const int i = i0 + (lane >> 1);
+    const int tile = min(2 * (first + wave + NW * i) + (lane & 1), last_tile);
+    const int e = tile / p.tpp;
+    place = tile - e * p.tpp;
+    id = i < mine ? table[e] : 0;
+  };
+  int id0, place0, id1, place1;   // of this 32 steps and of the next
+  entries(0, id0, place0);
+  entries(32, id1, place1);
 
   // the queries' fragments, channels in the codes' order; sums of channels and of bias * channel
   u32x4 qf[KW];
@@ -222,25 +264,60 @@ attn_decode_kernel(const AttnDecodeArgs p) {
 #pragma unroll
   for (int g = 0; g < NG; ++g) om[g] = 0.0f;
   float mx = -__builtin_inff(), l = 0.0f;
+  const uint32_t nibbles = code_mask();
   const u32x4 middle = u32x4{0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};   // -136
 
-  const int steps = (len + 31) / 32;
-  for (int st = lo / 32 + wave; st < steps; st += kDecodeWaves) {
+  struct Step {
     u32x4 kw[2], vw[2];
-    uint32_t kp[2][4 * NG], vp[2][4 * NG];
+    uint32_t pw[NG];   // lane: token lane % 32, of keys (lanes under 32) or values
+    int known;         // bit t: tile t's page exists
+  };
+  const char* const params = static_cast<const char*>(lane < 32 ? p.cache_kp : p.cache_vp) + (lane & 15) * (4 * NG);
+  const int koff = r * (D / 2) + q * (D / 8), voff = (r * 16 + 4 * q) * (D / 32);
+  auto load = [&](Step& f, int i) __attribute__((always_inline)) {   // i < mine
+    if (i > 0 && i % 32 == 0) {
+      id0 = id1;
+      place0 = place1;
+      entries(i + 32, id1, place1);
+    }
+    f.known = 0;
+    int64_t row[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      int tile = 2 * st + t;
-      if (tile * 16 >= len) tile = 2 * st;   // past the end: any tile that is there
-      int64_t page = table[tile / p.tpp];
-      if (page < 0 || page >= p.pages) page = 0;   // (its tokens are masked below)
-      const int64_t row = (page * p.kv + kvh) * p.tpp * 16 + (int64_t)(tile % p.tpp) * 16;
-      const uint8_t* kc = static_cast<const uint8_t*>(p.cache_kc) + (row + r) * (D / 2) + q * (D / 8);
-      const uint8_t* vc = static_cast<const uint8_t*>(p.cache_vc) + row * (D / 2) + (r * 16 + 4 * q) * (D / 32);
-      __builtin_memcpy(&kw[t], __builtin_assume_aligned(kc, D / 8), D / 8);
-      __builtin_memcpy(&vw[t], __builtin_assume_aligned(vc, D / 8), D / 8);
-      __builtin_memcpy(kp[t], __builtin_assume_aligned(static_cast<const uint32_t*>(p.cache_kp) + (row + 4 * q) * NG, 16), 16 * NG);
-      __builtin_memcpy(vp[t], __builtin_assume_aligned(static_cast<const uint32_t*>(p.cache_vp) + (row + 4 * q) * NG, 16), 16 * NG);
+      int page = __builtin_amdgcn_readlane(id0, 2 * (i % 32) + t);
+      const int place = __builtin_amdgcn_readlane(place0, 2 * (i % 32) + t);
+      if (page >= 0 && page < p.pages) f.known |= 1 << t;
+      else page = 0;   // (its tokens are masked)
+      row[t] = (((int64_t)page * p.kv + kvh) * p.tpp + place) * 16;
+      const char* kc = static_cast<const char*>(p.cache_kc) + row[t] * (D / 2) + koff;
+      const char* vc = static_cast<const char*>(p.cache_vc) + row[t] * (D / 2) + voff;
+      __builtin_memcpy(&f.kw[t], __builtin_assume_aligned(kc, D / 8), D / 8);
+      __builtin_memcpy(&f.vw[t], __builtin_assume_aligned(vc, D / 8), D / 8);
+    }
+    __builtin_memcpy(f.pw, __builtin_assume_aligned(params + ((lane & 16) ? row[1] : row[0]) * (4 * NG), 4 * NG), 4 * NG);
+  };
+  auto sum = [&](Step& f, int i) __attribute__((always_inline)) {
+    const int st = first + wave + NW * i;
+    // (a wave's LDS accesses are in order)
+    if (lane < 32) {
+      __builtin_memcpy(__builtin_assume_aligned(&spread_k[wave][lane * NG], 4 * NG), f.pw, 4 * NG);
+    } else {
+      float sc[NG], mid[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        sc[g] = f16_lo(f.pw[g]);
+        mid[g] = __builtin_fmaf(8.0f, sc[g], f16_hi(f.pw[g]));
+      }
+      __builtin_memcpy(__builtin_assume_aligned(&spread_v[wave][0][(lane & 31) * NG], 4 * NG), sc, 4 * NG);
+      __builtin_memcpy(__builtin_assume_aligned(&spread_v[wave][1][(lane & 31) * NG], 4 * NG), mid, 4 * NG);
+    }
+    uint32_t kp[2][4 * NG];
+    float vs[2][4 * NG], vm[2][4 * NG];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      __builtin_memcpy(kp[t], __builtin_assume_aligned(&spread_k[wave][(16 * t + 4 * q) * NG], 16), 16 * NG);
+      __builtin_memcpy(vs[t], __builtin_assume_aligned(&spread_v[wave][0][(16 * t + 4 * q) * NG], 16), 16 * NG);
+      __builtin_memcpy(vm[t], __builtin_assume_aligned(&spread_v[wave][1][(16 * t + 4 * q) * NG], 16), 16 * NG);
     }
     float s[2][4];
 #pragma unroll
@@ -251,7 +328,7 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       for (int g = 0; g < NG; ++g) {
         f32x4 raw = f32x4{-qb[g], -qb[g], -qb[g], -qb[g]};
 #pragma unroll
-        for (int k = 0; k < SG; ++k) raw = mma16<T>(code_frag<T>(kw[t][g * SG + k]), qf[g * SG + k], raw);
+        for (int k = 0; k < SG; ++k) raw = mma16<T>(code_frag<T>(f.kw[t][g * SG + k], nibbles), qf[g * SG + k], raw);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t w = kp[t][j * NG + g];
@@ -261,33 +338,30 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       }
     }
     // tokens outside [lo, len), and of page entries that name no page
+    if (st * 32 < lo || st * 32 + 32 > len || f.known != 3) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int tile = 2 * st + t;
-      const int64_t page = tile * 16 < len ? table[tile / p.tpp] : 0;
-      const bool there = page >= 0 && page < p.pages;
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int token = tile * 16 + 4 * q + j;
-        if (!there || token < lo || token >= len) {
-          s[t][j] = -__builtin_inff();
+        for (int j = 0; j < 4; ++j) {
+          const int token = st * 32 + 16 * t + 4 * q + j;
+          if (!(f.known >> t & 1) || token < lo || token >= len) {
+            s[t][j] = -__builtin_inff();
 #pragma unroll
-          for (int g = 0; g < NG; ++g) vp[t][j * NG + g] = 0;   // whatever is there: 0 * it is 0
+            for (int g = 0; g < NG; ++g) vs[t][j * NG + g] = vm[t][j * NG + g] = 0.0f;   // whatever is there: 0 * it is 0
+          }
         }
-      }
     }
     float m = s[0][0];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = __builtin_fmaxf(m, s[j / 4][j % 4]);
-    m = __builtin_fmaxf(m, __shfl_xor(m, 16, 64));
-    m = __builtin_fmaxf(m, __shfl_xor(m, 32, 64));
+    for (int j = 1; j < 8; ++j) m = __builtin_fmaxf(m, s[j / 4][j % 4]);
+    m = max_quarters(m);
     const float now = __builtin_fmaxf(mx, m);
-    const float base = now == -__builtin_inff() ? 0.0f : now;
-    const float keep = __builtin_amdgcn_exp2f((mx - base) * p.c);
+    const float base = now == -__builtin_inff() ? 0.0f : now * p.c;
+    const float keep = __builtin_amdgcn_exp2f(__builtin_fmaf(mx, p.c, -base));
     mx = now;
     float pt[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) pt[j] = __builtin_amdgcn_exp2f((s[j / 4][j % 4] - base) * p.c);
+    for (int j = 0; j < 8; ++j) pt[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], p.c, -base));
     l *= keep;
 #pragma unroll
     for (int j = 0; j < 8; ++j) l += pt[j];
@@ -297,49 +371,53 @@ attn_decode_kernel(const AttnDecodeArgs p) {
     for (int g = 0; g < NG; ++g) {
       om[g] *= keep;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t w = vp[j / 4][(j % 4) * NG + g];
-        om[g] = __builtin_fmaf(pt[j], __builtin_fmaf(8.0f, f16_lo(w), f16_hi(w)), om[g]);
-      }
+      for (int j = 0; j < 8; ++j) om[g] = __builtin_fmaf(pt[j], vm[j / 4][(j % 4) * NG + g], om[g]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float w0 = pt[2 * j] * f16_lo(vp[j / 2][(2 * j % 4) * NG + g]);
-        const float w1 = pt[2 * j + 1] * f16_lo(vp[j / 2][(2 * j % 4 + 1) * NG + g]);
-        const uint32_t h = pack2<__bf16>(w0, w1);
-        hi[g][j] = h;
-        lw[g][j] = pack2<__bf16>(w0 - bf16_lo(h), w1 - bf16_hi(h));
+      for (int j = 0; j < 4; ++j) {   // a weight's upper half, and the rest of it rounded
+        const float w0 = pt[2 * j] * vs[j / 2][(2 * j % 4) * NG + g];
+        const float w1 = pt[2 * j + 1] * vs[j / 2][(2 * j % 4 + 1) * NG + g];
+        const uint32_t u0 = __builtin_bit_cast(uint32_t, w0), u1 = __builtin_bit_cast(uint32_t, w1);
+        hi[g][j] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+        lw[g][j] = pack2<__bf16>(w0 - __builtin_bit_cast(float, u0 & 0xffff0000u), w1 - __builtin_bit_cast(float, u1 & 0xffff0000u));
       }
       start[g] = mma16<__bf16>(middle, lw[g], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
       start[g] = mma16<__bf16>(middle, hi[g], start[g]);
     }
 #pragma unroll
     for (int i = 0; i < CI; ++i) {
-      u32x4 f;
+      u32x4 c;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {   // tokens 2 j, 2 j + 1 of the eight
         uint32_t x;
-        if constexpr (D == 128) {
-          const uint32_t a = vw[j / 2][2 * j % 4], c = vw[j / 2][2 * j % 4 + 1];
-          x = i < 4 ? (a & 0xffffu) | (c << 16) : (a >> 16) | (c & 0xffff0000u);
-        } else {
-          x = vw[j / 2][j % 2];
-        }
-        f[j] = ((x >> (4 * (i % 4))) & 0x000f000fu) | 0x43004300u;
+        if constexpr (D == 128)
+          x = __builtin_amdgcn_perm(f.vw[j / 2][2 * j % 4 + 1], f.vw[j / 2][2 * j % 4], i < 4 ? 0x05040100u : 0x07060302u);
+        else
+          x = f.vw[j / 2][j % 2];
+        c[j] = ((x >> (4 * (i % 4))) & nibbles) | 0x43004300u;
       }
       const int g = i * NG / CI;
-      const f32x4 add = mma16<__bf16>(f, hi[g], mma16<__bf16>(f, lw[g], start[g]));
+      const f32x4 add = mma16<__bf16>(c, hi[g], mma16<__bf16>(c, lw[g], start[g]));
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = __builtin_fmaf(o[i][j], keep, add[j]);
     }
+  };
+  constexpr int kRing = 2;
+  Step ring[kRing];
+#pragma unroll
+  for (int i = 0; i < kRing - 1; ++i)
+    if (i < mine) load(ring[i], i);
+  for (int i = 0; i < mine; i += kRing) {
+#pragma unroll
+    for (int k = 0; k < kRing; ++k) {
+      if (i + k >= mine) break;
+      if (i + k + kRing - 1 < mine) load(ring[(k + kRing - 1) % kRing], i + k + kRing - 1);
+      sum(ring[k], i + k);
+    }
   }
   // channel 4 q + j + 16 i of head r; the lanes of a head hold a part each of l and om
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = sum_quarters(l);
 #pragma unroll
-  for (int g = 0; g < NG; ++g) {
-    om[g] += __shfl_xor(om[g], 16, 64);
-    om[g] += __shfl_xor(om[g], 32, 64);
-  }
+  for (int g = 0; g < NG; ++g) om[g] = sum_quarters(om[g]);
 #pragma unroll
   for (int i = 0; i < CI; ++i) {
     const int g = i * NG / CI;
@@ -351,25 +429,98 @@ attn_decode_kernel(const AttnDecodeArgs p) {
     red_l[wave][r] = l;
   }
   __syncthreads();
-  for (int idx = threadIdx.x; idx < nh * D; idx += 64 * kDecodeWaves) {
+  const int64_t group = (int64_t)b * gridDim.x + blockIdx.x;   // (b, head block, key head)
+  float* part = p.part + group * p.ranges * (16 * (D + 2));   // [range][head][value, maximum, sum]
+  T* out = static_cast<T*>(p.out) + (int64_t)b * p.ldo + (int64_t)head0 * D;
+  for (int idx = threadIdx.x; idx < nh * D; idx += 64 * NW) {
     const int h = idx / D, ch = idx % D;
     float m = red_m[0][h];
 #pragma unroll
-    for (int w = 1; w < kDecodeWaves; ++w) m = __builtin_fmaxf(m, red_m[w][h]);
-    const float base = m == -__builtin_inff() ? 0.0f : m;
-    float sum = 0.0f, acc = 0.0f;
+    for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, red_m[w][h]);
+    const float base = m == -__builtin_inff() ? 0.0f : m * p.c;
+    float total_l = 0.0f, acc = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kDecodeWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f((red_m[w][h] - base) * p.c);
-      sum += f * red_l[w][h];
+    for (int w = 0; w < NW; ++w) {
+      const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(red_m[w][h], p.c, -base));
+      total_l += f * red_l[w][h];
       acc += f * red[w][h][ch];
     }
-    static_cast<T*>(p.out)[(int64_t)b * p.ldo + (int64_t)(head0 + h) * D + ch] = (T)(sum == 0.0f ? 0.0f : acc / sum);
+    if (ranges == 1) {
+      out[h * D + ch] = (T)(total_l == 0.0f ? 0.0f : acc / total_l);   // no token: zeros
+    } else {
+      float* to = part + (int64_t)(range * 16 + h) * (D + 2);
+      to[ch] = acc;
+      if (ch == 0) {
+        to[D] = m;
+        to[D + 1] = total_l;
+      }
+    }
   }
 }
 
+// A block adds the ranges of one head; the factors of all ranges first, then
+// 256 / D threads a channel, each a run of ranges, whose sums are added in order.
+template <class T, int D>
+__global__ void __launch_bounds__(256)
+attn_decode_merge_kernel(const AttnDecodeArgs p) {
+  constexpr int PARTS = 256 / D;
+  __shared__ float factor[kDecodeMaxRanges], wave_m[4], wave_l[4], sums[PARTS][D];
+  const int b = blockIdx.y, head = blockIdx.x, kvh = head / p.g, hb = (head - kvh * p.g) / 16, h = (head - kvh * p.g) % 16;
+  const Span span = span_of(p, b);
+  if (span.ranges == 1) return;   // written already
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int hbs = (p.g + 15) / 16;
+  const int64_t group = ((int64_t)b * hbs + hb) * p.kv + kvh;
+  const float* part = p.part + group * p.ranges * (16 * (D + 2)) + h * (D + 2);
+  constexpr int kStride = 16 * (D + 2);   // floats between ranges
+  float m = -__builtin_inff();
+  for (int k = threadIdx.x; k < span.ranges; k += 256) {
+    const float v = part[(int64_t)k * kStride + D];
+    factor[k] = v;
+    m = __builtin_fmaxf(m, v);
+  }
+  for (int i = 1; i < 64; i *= 2) m = __builtin_fmaxf(m, __shfl_xor(m, i, 64));
+  if (lane == 0) wave_m[wave] = m;
+  __syncthreads();
+  m = __builtin_fmaxf(__builtin_fmaxf(wave_m[0], wave_m[1]), __builtin_fmaxf(wave_m[2], wave_m[3]));
+  const float base = m == -__builtin_inff() ? 0.0f : m * p.c;
+  float l = 0.0f;
+  for (int k = threadIdx.x; k < span.ranges; k += 256) {
+    const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(factor[k], p.c, -base));
+    factor[k] = f;
+    l += f * part[(int64_t)k * kStride + D + 1];
+  }
+  for (int i = 1; i < 64; i *= 2) l += __shfl_xor(l, i, 64);
+  if (lane == 0) wave_l[wave] = l;
+  __syncthreads();
+  l = (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]);
+  const int ch = threadIdx.x % D, run = threadIdx.x / D, per = (span.ranges + PARTS - 1) / PARTS;
+  float acc = 0.0f;
+#pragma unroll 8
+  for (int k = run * per; k < min(span.ranges, (run + 1) * per); ++k) acc += factor[k] * part[(int64_t)k * kStride + ch];
+  sums[run][ch] = acc;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+#pragma unroll
+  for (int i = 1; i < PARTS; ++i) acc += sums[i][ch];
+  static_cast<T*>(p.out)[(int64_t)b * p.ldo + (int64_t)head * D + ch] = (T)(l == 0.0f ? 0.0f : acc / l);
+}
+
+// Ranges of the longest sequence a call may have, and steps of 32 tokens each:
+// two blocks a CU (the registers' limit) where the sequences are long enough,
+// and no range under four steps a wave, which the second launch would outweigh.
+void decode_plan(int64_t batch, int kv, int g, int64_t longest, bool split, int* ranges, int* chunk) {
+  const int64_t blocks = batch * kv * ((g + 15) / 16), steps = std::max<int64_t>(1, (longest + 31) / 32);
+  constexpr int64_t least = 4 * kDecodeWaves;
+  const int64_t n = split ? std::min<int64_t>(std::max<int64_t>(1, kDecodeBlocks / blocks), (steps + least - 1) / least) : 1;
+  static_assert(kDecodeBlocks <= kDecodeMaxRanges, "the merge holds a factor a range");
+  const int64_t per = (steps + n - 1) / n;
+  *chunk = (int)((per + kDecodeWaves - 1) / kDecodeWaves * kDecodeWaves);
+  *ranges = (int)((steps + *chunk - 1) / *chunk);
+}
+
 template <class T, int D> static hipError_t decode_d(int group, const AttnDecodeArgs& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.kv * ((p.g + 15) / 16)), (unsigned)p.batch), block(64 * kDecodeWaves);
+  const dim3 grid((unsigned)(p.kv * ((p.g + 15) / 16)), (unsigned)p.batch, (unsigned)p.ranges), block(64 * kDecodeWaves);
   switch (D / group) {
     case 1: hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, block, 0, st, p); break;
     case 2: hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, block, 0, st, p); break;
@@ -378,6 +529,8 @@ template <class T, int D> static hipError_t decode_d(int group, const AttnDecode
       [[fallthrough]];
     default: return hipErrorInvalidValue;
   }
+  if (p.ranges > 1)
+    hipLaunchKernelGGL((attn_decode_merge_kernel<T, D>), dim3((unsigned)(p.kv * p.g), grid.y), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 hipError_t run_attn_decode(int dtype, int dim, int group, const AttnDecodeArgs& p, hipStream_t st) {

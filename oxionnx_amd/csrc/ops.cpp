@@ -2530,6 +2530,17 @@ extern "C" int ohip_attn_decode(ohip_ctx* ctx, const ohip_attn_decode_desc* d, c
   p.c = d->scale * 1.4426950408889634f;
   std::lock_guard<std::mutex> lock(ctx->mu);
   ctx->counters.dispatches++;
+  const int64_t groups = d->batch * p.kv * ((p.g + 15) / 16), longest = std::min((int64_t)d->width * cache->page, d->window > 0 ? (int64_t)d->window + 31 : INT64_MAX);
+  const size_t each = (size_t)groups * 16 * (cache->head_dim + 2) * sizeof(float);   // bytes a range
+  decode_plan(d->batch, p.kv, p.g, longest, true, &p.ranges, &p.chunk);
+  if (p.ranges > 1 && scratch_frozen(ctx, ScratchPlan::rounded(each * p.ranges)))
+    decode_plan(d->batch, p.kv, p.g, longest, false, &p.ranges, &p.chunk);
+  if (p.ranges > 1) {
+    ScratchPlan plan;
+    const size_t at = plan.add(each * p.ranges);
+    if ((rc = scratch_reserve(ctx, plan.total()))) return rc;
+    p.part = static_cast<float*>(scratch_at(ctx, plan, at));
+  }
   hipError_t e = run_attn_decode(d->dtype, cache->head_dim, cache->group, p, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "ohip_attn_decode launch");
   return OHIP_OK;

@@ -88,7 +88,7 @@ template <> struct Q4Mma<_Float16> {
     off = __builtin_bit_cast(u32x4, v);
   }
   __device__ __forceinline__ u32x4 frag(uint32_t w) const {
-    return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, code_frag<_Float16>(w)) - __builtin_bit_cast(f16x8, off));
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, code_frag<_Float16>(w, code_mask())) - __builtin_bit_cast(f16x8, off));
   }
   __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<_Float16>& a, f32x4 c) const { return mma16<_Float16>(f, a.v, c); }
 };
@@ -98,7 +98,7 @@ template <> struct Q4Mma<__bf16> {
     const uint32_t b = __builtin_bit_cast(uint32_t, (float)-(128 + z)) >> 16;
     off = u32x4{b * 0x10001u, b * 0x10001u, b * 0x10001u, b * 0x10001u};
   }
-  __device__ __forceinline__ u32x4 frag(uint32_t w) const { return code_frag<__bf16>(w); }
+  __device__ __forceinline__ u32x4 frag(uint32_t w) const { return code_frag<__bf16>(w, code_mask()); }
   __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const {
     return mma16<__bf16>(f, a.v, mma16<__bf16>(off, a.v, c));
   }

@@ -51,7 +51,12 @@ struct AttnDecodeArgs {
   int width, tpp;              // table entries a sequence; tiles of 16 tokens a page
   int batch, kv, g, window;
   float c;                     // softmax scale times log2(e)
+  int ranges, chunk;           // blocks of the longest sequence and key head, steps of 32 tokens each
+  float* part;                 // ranges > 1: batch * kv * ceil(g / 16) * ranges * 16 * (dim + 2)
 };
+// The ranges for sequences of up to `longest` tokens; split: whether there may be more than one.
+constexpr int kDecodeBlocks = 512, kDecodeMaxRanges = 512;
+void decode_plan(int64_t batch, int kv, int g, int64_t longest, bool split, int* ranges, int* chunk);
 hipError_t run_attn_decode(int dtype, int dim, int group, const AttnDecodeArgs& p, hipStream_t st);
 
 struct AttnPrefillArgs {
@@ -106,14 +111,20 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast
 // T, elements in the order of channels 0, 4, 1, 5, 2, 6, 3, 7: a code in the
 // low mantissa bits of a power of two.  f16 biases 1024, 1024, 64, 64, twice
 // (a code four bits up in the mantissa of 64 is that code); bf16 128.
-template <class T> __device__ __forceinline__ u32x4 code_frag(uint32_t w) {
+// `mask`: 0x000f000f in a vector register (code_mask), so that mask and bias
+// are one instruction, whose other constant is the one scalar it may read.
+__device__ __forceinline__ uint32_t code_mask() {
+  uint32_t m = 0x000f000fu;
+  asm("" : "+v"(m));
+  return m;
+}
+template <class T> __device__ __forceinline__ u32x4 code_frag(uint32_t w, uint32_t mask) {
   if constexpr (std::is_same<T, _Float16>::value) {
-    const uint32_t h = w >> 8;
-    return u32x4{(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x54005400u, (h & 0x000f000fu) | 0x64006400u,
-                 (h & 0x00f000f0u) | 0x54005400u};
+    const uint32_t h = w >> 8, high = mask << 4;
+    return u32x4{(w & mask) | 0x64006400u, (w & high) | 0x54005400u, (h & mask) | 0x64006400u, (h & high) | 0x54005400u};
   } else {
-    return u32x4{(w & 0x000f000fu) | 0x43004300u, ((w >> 4) & 0x000f000fu) | 0x43004300u,
-                 ((w >> 8) & 0x000f000fu) | 0x43004300u, ((w >> 12) & 0x000f000fu) | 0x43004300u};
+    return u32x4{(w & mask) | 0x43004300u, ((w >> 4) & mask) | 0x43004300u, ((w >> 8) & mask) | 0x43004300u,
+                 ((w >> 12) & mask) | 0x43004300u};
   }
 }
 __device__ constexpr int kCodeOrder[8] = {0, 4, 1, 5, 2, 6, 3, 7};
@@ -131,6 +142,18 @@ __device__ __forceinline__ float sum_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
   const uint32_t a = r[0], b = r[1];
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// the largest of, and the sum over, the four lanes l % 16 + 16 i
+__device__ __forceinline__ float max_quarters(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = r[0], b = r[1];
+  return max_halves(__builtin_fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+}
+__device__ __forceinline__ float sum_quarters(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+  const uint32_t a = r[0], b = r[1];
+  return sum_halves(__builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
 }
 
 // Waits for all but the wave's last N loads and for its LDS reads, then the
