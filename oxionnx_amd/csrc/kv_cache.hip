@@ -5,141 +5,193 @@
 namespace ohip {
 
 // ------------------------------------------------------------------ append
-// Eight channels a thread, D / 8 threads a head; a row of heads is a token's
-// queries, keys and values.  Rotation, group extremes and codes in f32:
+// Eight channels a thread, D / 8 lanes a head; a block has 256 * 8 / D tokens
+// and walks a run of their rows (query heads, key heads, value heads), so the
+// angles are loaded once and a tile of 16 tokens' value codes is written by
+// one block.  Rotation, group extremes and codes in f32:
 //   (o1, o2) = (x1 c - x2 s, x2 c + x1 s)          products rounded one by one
 //   scale = f16((max - min) / 15), low = f16(min)  (kept finite)
 //   code = clamp(rint((x - low) / scale), 0, 15)   (a group without extent: 0)
+// Bound: memory (8191 tokens, 32 + 2 x 8 heads of 128: 46 us, 4.7 TB/s; with a
+// thread a row and its angles read for each head 139).
 __device__ __forceinline__ float finite_f16(float v) {
   return v != v ? v : __builtin_fminf(__builtin_fmaxf(v, -65504.0f), 65504.0f);
+}
+
+// the value of lane l ^ 1, l ^ 2, of the mirrored lane of its 8, of its 16
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v)));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kXor3 = 0x1b, kMirror8 = 0x141, kMirror16 = 0x140, kRotate8 = 0x128;
+
+// One step of a transposition of nibbles between lanes: those of index bit S
+// against bit S of the lane's index i.
+template <int S> __device__ __forceinline__ uint32_t swap_nibbles(uint32_t w, uint32_t x, int i) {
+  constexpr uint32_t m = S == 1 ? 0x0f0f0f0fu : S == 2 ? 0x00ff00ffu : 0x0000ffffu;
+  return i & S ? (w & ~m) | ((x & ~m) >> (4 * S)) : (w & m) | ((x & m) << (4 * S));
 }
 
 template <class T, int D>
 __global__ void __launch_bounds__(256)
 kv_append_kernel(const KvAppendArgs p) {
-  constexpr int LPH = D / 8;   // lanes a head
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPH;
+  constexpr int LPH = D / 8, TPB = 256 / LPH;   // lanes a head, tokens a block
   const int c = threadIdx.x % LPH;
-  const int rows = p.q_heads + 2 * p.kv;
-  const int64_t token = at / rows;
+  const int64_t token = (int64_t)blockIdx.x * TPB + threadIdx.x / LPH;
   const bool live = token < p.tokens;   // whole heads: a head's lanes agree
-  const int slot_head = live ? (int)(at % rows) : 0;
-  const int64_t tk = live ? token : 0;
-  const int kind = slot_head < p.q_heads ? 0 : slot_head < p.q_heads + p.kv ? 1 : 2;   // q, k, v
-  const int h = kind == 0 ? slot_head : kind == 1 ? slot_head - p.q_heads : slot_head - p.q_heads - p.kv;
-  const T* src = static_cast<const T*>(kind == 0 ? p.q : kind == 1 ? p.k : p.v) +
-                 tk * (kind == 0 ? p.ldq : kind == 1 ? p.ldk : p.ldv) + h * D + 8 * c;
-  T raw[8];
-  __builtin_memcpy(raw, __builtin_assume_aligned(src, 16), 16);
-  float x[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (float)raw[e];
+  const int64_t tk = live ? token : p.tokens - 1;
+  const int rows = p.q_heads + 2 * p.kv, per = (rows + gridDim.y - 1) / gridDim.y;
+  const int row0 = blockIdx.y * per, row1 = min(rows, row0 + per);
+  const T* const q = static_cast<const T*>(p.q) + tk * p.ldq + 8 * c;
+  const T* const k = static_cast<const T*>(p.k) + tk * p.ldk + 8 * c;
+  const T* const v = static_cast<const T*>(p.v) + tk * p.ldv + 8 * c;
+  auto fetch = [&](int row) __attribute__((always_inline)) -> u32x4 {   // row: uniform
+    const T* src = row < p.q_heads ? q + (int64_t)row * D
+                 : row < p.q_heads + p.kv ? k + (int64_t)(row - p.q_heads) * D : v + (int64_t)(row - p.q_heads - p.kv) * D;
+    u32x4 raw;
+    __builtin_memcpy(&raw, __builtin_assume_aligned(src, 16), 16);
+    return raw;
+  };
+  if (row0 >= row1) return;
+  u32x4 next = fetch(row0);
 
-  if (p.cos && kind != 2) {   // (uniform over a head)
+  // this lane's angles: its channel pairs' (four), or its eight channels'
+  float cs[8], sn[8];
+  const int half = p.rot / 16;   // lanes that half of the rotated channels takes
+  const bool turned = p.cos && row0 < p.q_heads + p.kv && (p.interleaved ? 8 * c < p.rot : c < 2 * half);
+  const bool low = c < half;
+  if (turned) {
     int64_t pos = p.positions[tk];
     pos = pos < 0 ? 0 : pos >= p.max_position ? p.max_position - 1 : pos;
-    const float* cs = p.cos + pos * (p.rot / 2);
-    const float* sn = p.sin + pos * (p.rot / 2);
-    if (p.interleaved) {
-      if (8 * c < p.rot) {
+    const int64_t at = pos * (p.rot / 2) + (p.interleaved ? 4 * c : 8 * (low ? c : c - half));
+    const int n = p.interleaved ? 4 : 8;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = x[2 * j], b = x[2 * j + 1], cv = cs[4 * c + j], sv = sn[4 * c + j];
-          x[2 * j] = a * cv - b * sv;
-          x[2 * j + 1] = b * cv + a * sv;
+    for (int e = 0; e < 8; ++e) {
+      cs[e] = e < n ? p.cos[at + e] : 0.0f;
+      sn[e] = e < n ? p.sin[at + e] : 0.0f;
+    }
+  }
+  const int mate = (threadIdx.x & 63) + (low ? half : -half);   // of a turned lane
+
+  // where the token's codes and parameters go
+  const int64_t slot = p.slots[tk], page = slot / p.page;
+  const bool kept = live && slot >= 0 && slot < p.pages * p.page;   // else a padding token
+  const int off = (int)(slot - page * p.page);
+  const int gl = p.group / 8;   // lanes a group: 4, 8 or 16
+
+  for (int row = row0; row < row1; ++row) {
+    const u32x4 raw = next;
+    if (row + 1 < row1) next = fetch(row + 1);
+    const int kind = row < p.q_heads ? 0 : row < p.q_heads + p.kv ? 1 : 2;   // q, k, v
+    const int h = row - (kind == 0 ? 0 : kind == 1 ? p.q_heads : p.q_heads + p.kv);
+    T in[8];
+    __builtin_memcpy(in, &raw, 16);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (float)in[e];
+    if (p.cos && kind != 2) {
+      if (p.interleaved) {
+        if (turned) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float a = x[2 * j], b = x[2 * j + 1];
+            x[2 * j] = a * cs[j] - b * sn[j];
+            x[2 * j + 1] = b * cs[j] + a * sn[j];
+          }
+        }
+      } else {
+        u32x4 theirs;   // the mate's eight channels as they came
+#pragma unroll
+        for (int i = 0; i < 4; ++i) theirs[i] = (uint32_t)__shfl((int)raw[i], mate, 64);
+        T other[8];
+        __builtin_memcpy(other, &theirs, 16);
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float own = x[e] * cs[e], cross = (float)other[e] * sn[e];
+            x[e] = low ? own - cross : own + cross;
+          }
         }
       }
-    } else {
-      const int half = p.rot / 16;   // lanes a half of the rotated channels takes
-      const bool low = c < half, in = c < 2 * half;
-      const int mate = (threadIdx.x & 63) + (in ? (low ? half : -half) : 0);
-      const int a0 = 8 * (low ? c : c - half);
+    }
+    if (kind != 0) {
+      // the group's extremes; a NaN makes the whole group NaN
+      float lo = x[0], hi = x[0];
+      bool bad = x[0] != x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) {
+        lo = __builtin_fminf(lo, x[e]);
+        hi = __builtin_fmaxf(hi, x[e]);
+        bad |= x[e] != x[e];
+      }
+      lo = __builtin_fminf(lo, dpp<kXor1>(lo));
+      hi = __builtin_fmaxf(hi, dpp<kXor1>(hi));
+      lo = __builtin_fminf(lo, dpp<kXor2>(lo));
+      hi = __builtin_fmaxf(hi, dpp<kXor2>(hi));
+      if (gl >= 8) {
+        lo = __builtin_fminf(lo, dpp<kMirror8>(lo));
+        hi = __builtin_fmaxf(hi, dpp<kMirror8>(hi));
+      }
+      if (gl >= 16) {
+        lo = __builtin_fminf(lo, dpp<kMirror16>(lo));
+        hi = __builtin_fmaxf(hi, dpp<kMirror16>(hi));
+      }
+      const uint64_t any = __ballot(bad);
+      if (any && ((any >> (threadIdx.x & 63 & ~(gl - 1))) & ((1u << gl) - 1))) lo = hi = __builtin_nanf("");
+      const _Float16 s16 = (_Float16)finite_f16((hi - lo) * (1.0f / 15.0f)), l16 = (_Float16)finite_f16(lo);
+      const float sc = (float)s16, lw = (float)l16;
+      uint32_t word = 0;   // nibble e: channel 8 c + e
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float other = __shfl(x[e], mate, 64);
-        if (in) {
-          const float cv = cs[a0 + e], sv = sn[a0 + e];
-          x[e] = low ? x[e] * cv - other * sv : x[e] * cv + other * sv;
+        const float t = sc > 0.0f ? __builtin_rintf((x[e] - lw) / sc) : 0.0f;
+        const uint32_t code = t >= 15.0f ? 15u : t > 0.0f ? (uint32_t)t : 0u;
+        word |= code << (4 * e);
+        if (p.held) x[e] = (float)code * sc + lw;
+      }
+      const int64_t at = (page * p.kv + h) * p.page + off;   // the token's row of the head
+      if (kept && c % gl == 0)
+        static_cast<uint32_t*>(kind == 1 ? p.cache_kp : p.cache_vp)[at * (D / p.group) + c / gl] =
+            (uint32_t)__builtin_bit_cast(uint16_t, s16) | (uint32_t)__builtin_bit_cast(uint16_t, l16) << 16;
+      if (kind == 1) {   // word of channels 32 s + 8 q ..: [q][s]
+        if (kept) static_cast<uint32_t*>(p.cache_kc)[at * (D / 8) + (c & 3) * (D / 32) + (c >> 2)] = word;
+      } else {
+        // A value column o holds the channels o + 16 i, which lane 2 i + o / 8
+        // has as its nibble o % 8: a transposition among the lanes of one
+        // parity, after which lane 2 i + h has column(s) 8 h + i (and 8 h + i + 4).
+        const int i = c >> 1;
+        word = swap_nibbles<1>(word, dpp<kXor2>(word), i);
+        word = swap_nibbles<2>(word, dpp<kXor3>(dpp<kMirror8>(word)), i);   // lane ^ 4
+        if constexpr (D == 128) word = swap_nibbles<4>(word, dpp<kRotate8>(word), i);
+        if (kept) {
+          char* to = static_cast<char*>(p.cache_vc) + (at - (off & 15)) * (D / 2) + ((8 * (c & 1) + i) * 16 + (off & 15)) * (D / 32);
+          if constexpr (D == 128) {
+            *reinterpret_cast<uint32_t*>(to) = word;
+          } else {
+            *reinterpret_cast<uint16_t*>(to) = (uint16_t)word;
+            *reinterpret_cast<uint16_t*>(to + 4 * 16 * (D / 32)) = (uint16_t)(word >> 16);
+          }
         }
       }
     }
-  }
-  T* out = static_cast<T*>(kind == 0 ? p.q_out : kind == 1 ? p.k_out : p.v_out);
-  const int64_t ldo = kind == 0 ? p.ldqo : kind == 1 ? p.ldko : p.ldvo;
-
-  // the group's extremes (NaN is kept: a group with one stands for NaN)
-  float lo = x[0], hi = x[0];
-  bool nan = false;
+    T* out = static_cast<T*>(kind == 0 ? p.q_out : kind == 1 ? p.k_out : p.v_out);
+    if (out && live) {
+      const int64_t ldo = kind == 0 ? p.ldqo : kind == 1 ? p.ldko : p.ldvo;
+      T e8[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = __builtin_fminf(lo, x[e]);
-    hi = __builtin_fmaxf(hi, x[e]);
-    nan |= x[e] != x[e];
-  }
-  const int gl = p.group / 8;   // lanes a group: 4, 8 or 16, a power of two
-  for (int m = 1; m < gl; m *= 2) {
-    lo = __builtin_fminf(lo, __shfl_xor(lo, m, 64));
-    hi = __builtin_fmaxf(hi, __shfl_xor(hi, m, 64));
-    nan |= __shfl_xor((int)nan, m, 64) != 0;
-  }
-  if (nan) lo = hi = __builtin_nanf("");
-  const _Float16 s16 = (_Float16)finite_f16((hi - lo) * (1.0f / 15.0f)), l16 = (_Float16)finite_f16(lo);
-  const float sc = (float)s16, lw = (float)l16;
-  uint32_t word = 0;   // nibble e: channel 8 c + e
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float v = sc > 0.0f ? __builtin_rintf((x[e] - lw) / sc) : 0.0f;
-    const uint32_t code = v >= 15.0f ? 15u : v > 0.0f ? (uint32_t)v : 0u;
-    word |= code << (4 * e);
-    if (kind != 0 && p.held) x[e] = (float)code * sc + lw;
-  }
-  // a value column holds the channels o + 16 i: nibble i from the lane of channel 16 i + o
-  uint32_t col[16 / LPH];
-#pragma unroll
-  for (int t = 0; t < 16 / LPH; ++t) {
-    const int o = c + t * LPH;
-    col[t] = 0;
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const uint32_t w = (uint32_t)__shfl((int)word, (threadIdx.x & 63) - c + 2 * i + (o >> 3), 64);
-      col[t] |= ((w >> (4 * (o & 7))) & 15u) << (4 * i);
-    }
-  }
-  if (!live) return;
-  if (out) {
-    T e8[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) e8[e] = (T)x[e];
-    __builtin_memcpy(__builtin_assume_aligned(out + tk * ldo + h * D + 8 * c, 16), e8, 16);
-  }
-  if (kind == 0) return;
-  const int64_t slot = p.slots[tk];
-  if (slot < 0 || slot >= p.pages * p.page) return;   // a padding token
-  const int64_t page = slot / p.page;
-  const int off = (int)(slot - page * p.page);
-  const int64_t row = (page * p.kv + h) * p.page + off;   // this token's row of the head
-  uint32_t* params = reinterpret_cast<uint32_t*>(kind == 1 ? p.cache_kp : p.cache_vp);
-  if (c % gl == 0)
-    params[row * (D / p.group) + c / gl] =
-        (uint32_t)__builtin_bit_cast(uint16_t, s16) | (uint32_t)__builtin_bit_cast(uint16_t, l16) << 16;
-  if (kind == 1) {
-    // word of channels 32 s + 8 q ..: [q][s]
-    reinterpret_cast<uint32_t*>(p.cache_kc)[row * (D / 8) + (c & 3) * (D / 32) + (c >> 2)] = word;
-  } else {
-    uint8_t* tile = static_cast<uint8_t*>(p.cache_vc) + (row - (off & 15)) * (D / 2);
-#pragma unroll
-    for (int t = 0; t < 16 / LPH; ++t) {
-      const int o = c + t * LPH;
-      uint8_t* to = tile + (o * 16 + (off & 15)) * (D / 32);
-      if constexpr (D == 128) *reinterpret_cast<uint32_t*>(to) = col[t];
-      else *reinterpret_cast<uint16_t*>(to) = (uint16_t)col[t];
+      for (int e = 0; e < 8; ++e) e8[e] = (T)x[e];
+      __builtin_memcpy(__builtin_assume_aligned(out + tk * ldo + h * D + 8 * c, 16), e8, 16);
     }
   }
 }
 
 template <class T> static hipError_t append_t(int dim, const KvAppendArgs& p, hipStream_t st) {
-  const int64_t threads = p.tokens * (p.q_heads + 2 * p.kv) * (dim / 8);
-  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+  const int64_t per_block = 256 * 8 / dim, tiles = (p.tokens + per_block - 1) / per_block;
+  // rows a block: all of a token's where there are enough tokens for 1024 blocks
+  const int rows = p.q_heads + 2 * p.kv;
+  const int64_t runs = std::min<int64_t>(rows, std::max<int64_t>(1, (1024 + tiles - 1) / tiles));
+  const dim3 grid((unsigned)tiles, (unsigned)runs), block(256);
   if (dim == 128) hipLaunchKernelGGL((kv_append_kernel<T, 128>), grid, block, 0, st, p);
   else if (dim == 64) hipLaunchKernelGGL((kv_append_kernel<T, 64>), grid, block, 0, st, p);
   else return hipErrorInvalidValue;

@@ -82,23 +82,25 @@ template <> struct Act<float> { float v[8]; };
 template <class T> struct Q4Mma;
 template <> struct Q4Mma<_Float16> {
   u32x4 off;   // (1024 + z) twice, (64 + z) twice
+  uint32_t mask = code_mask();
   __device__ __forceinline__ void zero(int z) {
     const _Float16 a = (_Float16)(1024 + z), b = (_Float16)(64 + z);
     const f16x8 v = {a, a, b, b, a, a, b, b};
     off = __builtin_bit_cast(u32x4, v);
   }
   __device__ __forceinline__ u32x4 frag(uint32_t w) const {
-    return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, code_frag<_Float16>(w, code_mask())) - __builtin_bit_cast(f16x8, off));
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(f16x8, code_frag<_Float16>(w, mask)) - __builtin_bit_cast(f16x8, off));
   }
   __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<_Float16>& a, f32x4 c) const { return mma16<_Float16>(f, a.v, c); }
 };
 template <> struct Q4Mma<__bf16> {
   u32x4 off;
+  uint32_t mask = code_mask();
   __device__ __forceinline__ void zero(int z) {
     const uint32_t b = __builtin_bit_cast(uint32_t, (float)-(128 + z)) >> 16;
     off = u32x4{b * 0x10001u, b * 0x10001u, b * 0x10001u, b * 0x10001u};
   }
-  __device__ __forceinline__ u32x4 frag(uint32_t w) const { return code_frag<__bf16>(w, code_mask()); }
+  __device__ __forceinline__ u32x4 frag(uint32_t w) const { return code_frag<__bf16>(w, mask); }
   __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const {
     return mma16<__bf16>(f, a.v, mma16<__bf16>(off, a.v, c));
   }
@@ -121,65 +123,103 @@ template <> struct Q4Mma<float> {
   }
 };
 
-constexpr int kQ4Waves = 8;
-
-// A block takes 16 rows of the weight; its eight waves split K and meet in
-// LDS in wave order.  GS: steps of 32 k a group holds (four for any larger).
-template <class T, int TM, int GS>
-__global__ void __launch_bounds__(64 * kQ4Waves)
+// A block takes 16 rows of the weight; its NW waves split K and meet in LDS in
+// wave order.  GS: steps of 32 k a group holds (four for any larger).
+// Bound: streaming the weight once, and for more rows the activations' traffic
+// from L2 (M * K elements a block).  Both need loads in flight: a ring of
+// tiles of 128 k of codes, and the next tile's activations.
+template <class T, int TM, int GS, int NW>
+__global__ void __launch_bounds__(64 * NW, NW / 4)
 q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes, const T* __restrict__ scales,
           const uint8_t* __restrict__ zp, int M, int N, int K, int group, const FloatEpi<T> epi) {
-  __shared__ f32x4 red[kQ4Waves][TM][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ f32x4 red[NW][TM][64];
+  constexpr int GN = 4 / GS;   // groups of a tile
+  // (what the registers hold: a tile of activations is 8 TM registers of f16, 16 of f32)
+  constexpr int kRing = TM * sizeof(T) <= 4 ? 4 : 2, kActs = TM * sizeof(T) <= 4 ? 2 : 1;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int KT = (K + 127) / 128, blocks = (K + group - 1) / group;
-  const int per = (KT + kQ4Waves - 1) / kQ4Waves;
-  const int t0 = wave * per, t1 = min(t0 + per, KT);
-  const u32x4* wt = codes + (int64_t)blockIdx.x * KT * 64 + lane;
-  const T* sc = scales + (int64_t)blockIdx.x * blocks * 16;
-  const uint8_t* zr = zp ? zp + (int64_t)blockIdx.x * blocks * 16 : nullptr;
-  const T* ar[TM];
+  const int shift = GS == 1 ? 5 : GS == 2 ? 6 : group == 256 ? 8 : 7;   // log2(group)
+  const int KT = (K + 127) / 128, blocks = (K + (1 << shift) - 1) >> shift;
+  const int per = (KT + NW - 1) / NW;
+  const int t0 = wave * per, mine = max(0, min(per, KT - t0));
+  const u32x4* wt = codes + ((int64_t)blockIdx.x * KT + t0) * 64 + lane;
+  const T* sc = scales + (int64_t)blockIdx.x * blocks * 16 + 4 * q;
+  const uint8_t* zr = zp ? zp + (int64_t)blockIdx.x * blocks * 16 + r : nullptr;
+  const T* ar[TM];   // (columns past M are not stored)
 #pragma unroll
-  for (int t = 0; t < TM; ++t) ar[t] = a + (int64_t)min(t * 16 + r, M - 1) * lda;
+  for (int t = 0; t < TM; ++t) ar[t] = a + (int64_t)min(t * 16 + r, M - 1) * lda + 8 * q;
   f32x4 acc[TM];
 #pragma unroll
   for (int t = 0; t < TM; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int kt = t0; kt < t1; ++kt) {
-    const u32x4 w = wt[(int64_t)kt * 64];
-    f32x4 raw[TM];
-    Q4Mma<T> mul;
+  struct Tile {
+    u32x4 w;
+    T s[GN][4];
+    uint8_t z[GN];
+  };
+  struct Acts { Act<T> x[4][TM]; };
+  auto load = [&](Tile& f, int i) __attribute__((always_inline)) {   // i < mine
+    f.w = wt[(int64_t)i * 64];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int k = kt * 128 + s * 32 + 8 * q;
-      const int b = min((kt * 128 + s * 32) / group, blocks - 1);
-      if (s % GS == 0) {
-        mul.zero(zr ? zr[(int64_t)b * 16 + r] : 8);
+    for (int g = 0; g < GN; ++g) {
+      const int b = min(((t0 + i) * 128 + 32 * GS * g) >> shift, blocks - 1);
+      __builtin_memcpy(f.s[g], __builtin_assume_aligned(sc + (int64_t)b * 16, 4 * sizeof(T)), 4 * sizeof(T));
+      f.z[g] = zr ? zr[(int64_t)b * 16] : 8;
+    }
+  };
+  auto load_acts = [&](Acts& f, int i) __attribute__((always_inline)) {
+    const int kt = t0 + i;
+    if (kt * 128 + 128 <= K) {
 #pragma unroll
-        for (int t = 0; t < TM; ++t) raw[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      }
-      const auto f = mul.frag(w[s]);
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int t = 0; t < TM; ++t) {
-        Act<T> x;
-        if (k + 8 <= K && t * 16 + r < M) {
-          __builtin_memcpy(&x, ar[t] + k, sizeof(x));
-        } else {
+        for (int t = 0; t < TM; ++t) __builtin_memcpy(&f.x[s][t], ar[t] + (kt * 128 + 32 * s), sizeof(f.x[s][t]));
+    } else {   // the rows' end
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int t = 0; t < TM; ++t) {
+          const int k = kt * 128 + 32 * s;
           T e[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) e[i] = t * 16 + r < M && k + i < K ? ar[t][k + i] : T(0);
-          __builtin_memcpy(&x, e, sizeof(x));
+          for (int j = 0; j < 8; ++j) e[j] = k + 8 * q + j < K ? ar[t][k + j] : T(0);
+          __builtin_memcpy(&f.x[s][t], e, sizeof(f.x[s][t]));
         }
-        raw[t] = mul.mma(f, x, raw[t]);
+    }
+  };
+  auto sum = [&](const Tile& f, const Acts& x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < GN; ++g) {
+      Q4Mma<T> mul;
+      mul.zero(f.z[g]);
+      f32x4 raw[TM];
+#pragma unroll
+      for (int t = 0; t < TM; ++t) raw[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < GS; ++s) {
+        const auto c = mul.frag(f.w[g * GS + s]);
+#pragma unroll
+        for (int t = 0; t < TM; ++t) raw[t] = mul.mma(c, x.x[g * GS + s][t], raw[t]);
       }
-      if (s % GS == GS - 1) {
-        f32x4 sv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sv[i] = to_f32(sc[(int64_t)b * 16 + 4 * q + i]);
+      for (int t = 0; t < TM; ++t)
 #pragma unroll
-        for (int t = 0; t < TM; ++t)
+        for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(to_f32(f.s[g][i]), raw[t][i], acc[t][i]);
+    }
+  };
+  Tile ring[kRing];
+  Acts acts[kActs];
+  if (kActs > 1 && mine > 0) load_acts(acts[0], 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_fmaf(sv[i], raw[t][i], acc[t][i]);
-      }
+  for (int i = 0; i < kRing - 1; ++i)
+    if (i < mine) load(ring[i], i);
+  for (int i = 0; i < mine; i += kRing) {
+#pragma unroll
+    for (int k = 0; k < kRing; ++k) {
+      if (i + k >= mine) break;
+      // (the activations first: loads arrive in order, and these are waited for next)
+      if (i + k + kActs - 1 < mine) load_acts(acts[(k + kActs - 1) % kActs], i + k + kActs - 1);
+      if (i + k + kRing - 1 < mine) load(ring[(k + kRing - 1) % kRing], i + k + kRing - 1);
+      sum(ring[k], acts[k % kActs]);
     }
   }
 #pragma unroll
@@ -188,7 +228,7 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
   if (wave >= TM) return;
   f32x4 v = red[0][wave][lane];
 #pragma unroll
-  for (int k = 1; k < kQ4Waves; ++k) v += red[k][wave][lane];
+  for (int k = 1; k < NW; ++k) v += red[k][wave][lane];
   const int i = blockIdx.x * 16 + 4 * q, j = wave * 16 + r;
   if (j >= M || i >= N) return;
   typename FloatEpi<T>::PreI pi;
@@ -201,19 +241,28 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
   store_group(out, epi.out_bytes(), out.row(i), i, j, bits);
 }
 
-template <class T, int TM>
-static hipError_t q4_t(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
+template <class T, int TM, int NW>
+static hipError_t q4_w(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
   const T* a = static_cast<const T*>(g.a);
   const u32x4* codes = static_cast<const u32x4*>(g.codes);
   const T* sc = static_cast<const T*>(g.scales);
-  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * kQ4Waves);
+  const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * NW);
   if (g.group == 32)
-    hipLaunchKernelGGL((q4_kernel<T, TM, 1>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 1, NW>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
   else if (g.group == 64)
-    hipLaunchKernelGGL((q4_kernel<T, TM, 2>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 2, NW>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
   else
-    hipLaunchKernelGGL((q4_kernel<T, TM, 4>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 4, NW>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
   return hipGetLastError();
+}
+// Four waves a block where there are two blocks a CU, which then hold all of
+// the launch at once (1 x 4096 x 11008 f16, 688 blocks: 8.9 us, eight waves
+// 9.5); else eight (16 x 11008 x 4096 bf16, 256 blocks: 14.8, four 17.5,
+// sixteen 14.9).
+template <class T, int TM> static hipError_t q4_t(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
+  if constexpr (TM * sizeof(T) <= 4)
+    if (g.N >= 512 * 16) return q4_w<T, TM, 4>(g, epi, st);
+  return q4_w<T, TM, 8>(g, epi, st);
 }
 
 template <class T> static hipError_t q4_m(const Q4Args& g, const FloatOut& o, hipStream_t st) {

@@ -100,20 +100,17 @@ def _invalid(msg):
 def _heads(t, name, dtype, device):
     """Checks [tokens, heads, channels] of a 16-bit `dtype` on GPU `device`, heads next to each other;
     the elements between tokens."""
-    if t.dtype != dtype or t.get_device() != device:
-        raise _invalid(f"{name}: {dtype} on GPU {device} is expected")
-    try:
-        rows, per_head, one = t.stride()
-    except ValueError:
-        raise _invalid(f"{name}: [tokens, heads, channels] is expected") from None
-    _, heads, dim = t.shape
-    if (one != 1 and dim > 1) or (per_head != dim and heads > 1):
+    strides = t.stride()
+    if t.dtype != dtype or t.get_device() != device or len(strides) != 3:
+        raise _invalid(f"{name}: [tokens, heads, channels] of {dtype} on GPU {device} is expected")
+    tokens, heads, dim = t.shape
+    if (strides[2] != 1 and dim > 1) or (strides[1] != dim and heads > 1):
         raise _invalid(f"{name}: a token's heads are not next to each other")
-    return rows if t.shape[0] > 1 else heads * dim
+    return strides[0] if tokens > 1 else heads * dim
 
 
 def _table(t, name, dtype, device, shape):
-    if t.dtype != dtype or t.get_device() != device or not t.is_contiguous() or t.shape != shape:
+    if t.dtype != dtype or t.get_device() != device or t.shape != shape or not t.is_contiguous():
         raise _invalid(f"{name}: a contiguous {dtype} array of {tuple(shape)} on GPU {device} is expected")
     return t.data_ptr()
 
@@ -534,49 +531,50 @@ class HipContext:
         not written), keys and queries rotated by rows `positions` (int32) of cos / sin (float32 [positions,
         rot / 2]); see ohip_kv_append.  Returns (q_out, k_out, v_out): the rotated queries, and keys and values
         as the cache holds them (out_held) or as they went in; k_out / v_out False: not wanted."""
-        torch = _torch()
-        at, dt, f32, i32 = self.device, k.dtype, torch.float32, torch.int32
-        tokens, kv, dim = k.shape if k.dim() == 3 else (0, 0, 0)
-        if kv != cache.kv_heads or dim != cache.dim or v.shape != k.shape or cache.device != at:
+        at, dt = self.device, k.dtype
+        shape = k.shape
+        if len(shape) != 3 or v.shape != shape or shape[1] != cache.kv_heads or shape[2] != cache.dim or cache.device != at:
             raise _invalid("kv_append: keys and values [tokens, kv_heads, dim] of the cache")
+        tokens, kv, dim = shape
         ldk, ldv = _heads(k, "kv_append: k", dt, at), _heads(v, "kv_append: v", dt, at)
-        heads, ldq, ldqo, rot, rows = 0, 0, 0, 0, 0
+        heads = ldq = ldqo = ldko = ldvo = rot = rows = 0
+        qp = qop = kop = vop = pos = cs = sn = None
         if q is not None:
-            if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim:
+            qshape = q.shape
+            if len(qshape) != 3 or qshape[0] != tokens or qshape[2] != dim:
                 raise _invalid("kv_append: q [tokens, heads, dim]")
-            heads, ldq = q.shape[1], _heads(q, "kv_append: q", dt, at)
+            heads, ldq = qshape[1], _heads(q, "kv_append: q", dt, at)
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=dt, device=q.device)
-            elif q_out.shape != q.shape:
+                q_out = _torch().empty(qshape, dtype=dt, device=q.device)
+            elif q_out.shape != qshape:
                 raise _invalid("kv_append: q_out has another shape than q")
-            ldqo = _heads(q_out, "kv_append: q_out", dt, at)
-        ld = []
-        outs = []
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t is False:
-                ld.append(0)
-                outs.append(None)
-                continue
-            if t is None:
-                t = torch.empty(k.shape, dtype=dt, device=k.device)
-            elif t.shape != k.shape:
-                raise _invalid(f"kv_append: {name} has another shape than k")
-            ld.append(_heads(t, name, dt, at))
-            outs.append(t)
-        pos = cs = sn = None
+            ldqo, qp, qop = _heads(q_out, "kv_append: q_out", dt, at), q.data_ptr(), q_out.data_ptr()
+        if k_out is None:
+            k_out = _torch().empty(shape, dtype=dt, device=k.device)
+        if k_out is not False:
+            if k_out.shape != shape:
+                raise _invalid("kv_append: k_out has another shape than k")
+            ldko, kop = _heads(k_out, "kv_append: k_out", dt, at), k_out.data_ptr()
+        if v_out is None:
+            v_out = _torch().empty(shape, dtype=dt, device=k.device)
+        if v_out is not False:
+            if v_out.shape != shape:
+                raise _invalid("kv_append: v_out has another shape than k")
+            ldvo, vop = _heads(v_out, "kv_append: v_out", dt, at), v_out.data_ptr()
+        i32 = _TORCH_DT[L.I32]
         if cos is not None:
-            rows, rot = cos.shape[0], 2 * cos.shape[1]
-            cs = _table(cos, "kv_append: cos", f32, at, cos.shape)
-            sn = _table(sin, "kv_append: sin", f32, at, cos.shape)
+            f32, angles = _TORCH_DT[L.F32], cos.shape
+            if len(angles) != 2:
+                raise _invalid("kv_append: cos [positions, rot / 2]")
+            rows, rot = angles[0], 2 * angles[1]
+            cs, sn = _table(cos, "kv_append: cos", f32, at, angles), _table(sin, "kv_append: sin", f32, at, angles)
             pos = _table(positions, "kv_append: positions", i32, at, (tokens,))
-        d = _KV_APPEND(tokens, ohip_dtype(dt), heads, rot, int(interleaved), int(out_held), rows, ldq, ldk, ldv, ldqo,
-                       ld[0], ld[1])
-        rc = L.raw("ohip_kv_append")(self.h, d, cache.desc, _ptr(q), k.data_ptr(), v.data_ptr(), pos, cs, sn,
-                                     _table(slots, "kv_append: slots", i32, at, (tokens,)), _ptr(q_out),
-                                     _ptr(outs[0]), _ptr(outs[1]))
+        d = _KV_APPEND(tokens, ohip_dtype(dt), heads, rot, interleaved, out_held, rows, ldq, ldk, ldv, ldqo, ldko, ldvo)
+        rc = L.raw("ohip_kv_append")(self.h, d, cache.desc, qp, k.data_ptr(), v.data_ptr(), pos, cs, sn,
+                                     _table(slots, "kv_append: slots", i32, at, (tokens,)), qop, kop, vop)
         if rc:
             L.check(rc)
-        return q_out, outs[0], outs[1]
+        return q_out, (None if k_out is False else k_out), (None if v_out is False else v_out)
 
     def attn_decode(self, q, cache, table, lens, scale=None, window=0, out=None):
         """Attention of one query token a sequence [batch, heads, dim] over the first lens[b] (int32) tokens of
