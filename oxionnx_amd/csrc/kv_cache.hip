@@ -223,6 +223,11 @@ hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t 
 // O^T = V^T P^T wants its right operand when the values' tokens are counted
 // 4 q + j of the first tile, then of the second.
 //
+// Up to eight heads leave half of the sixteen columns free: then (P = 2) a
+// column is a head of one of the two tiles, so that a lane has the softmax of
+// four tokens instead of eight; the columns of the other tile get no weight,
+// and each column keeps a maximum and sums of its own until the end.
+//
 // Ranges of one sequence leave their maxima, sums and weighted values in `part`;
 // a second launch adds them in order.  (Counting the blocks and letting the
 // last one add saves the launch, but its fences write back and invalidate an
@@ -242,14 +247,16 @@ __device__ __forceinline__ Span span_of(const AttnDecodeArgs& p, int b) {
   return s;
 }
 
-template <class T, int D, int NG>
-__global__ void __launch_bounds__(64 * kDecodeWaves, NG == 4 ? 1 : 2)
+template <class T, int D, int NG, int P>
+__global__ void __launch_bounds__(64 * kDecodeWaves, NG == 4 && P == 1 ? 1 : 2)
 attn_decode_kernel(const AttnDecodeArgs p) {
   constexpr int NW = kDecodeWaves;
   constexpr int KW = D / 32;   // steps of 32 channels
   constexpr int CI = D / 16;   // channels of a value column
   constexpr int SG = KW / NG;  // steps a group
   constexpr int RS = D + 4;
+  constexpr int HC = 16 / P;   // heads of the columns
+  constexpr int VS = 2 / P;    // tiles of a lane's columns
   __shared__ float red[NW][16][RS];
   __shared__ float red_m[NW][16], red_l[NW][16];
   // of a wave's step, [token][group]: the keys' pairs, the values' scales and middles (of code 8)
@@ -258,8 +265,9 @@ attn_decode_kernel(const AttnDecodeArgs p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int b = blockIdx.y, kvh = blockIdx.x % p.kv, hb = blockIdx.x / p.kv;
-  const int nh = min(16, p.g - hb * 16);   // query heads of this block
-  const int head0 = kvh * p.g + hb * 16;
+  const int nh = min(HC, p.g - hb * HC);   // query heads of this block
+  const int head0 = kvh * p.g + hb * HC;
+  const int hr = r % HC, half = r / HC;    // this lane's head, and tile if P = 2
   const Span span = span_of(p, b);
   const int len = span.len, lo = span.lo, ranges = span.ranges, range = blockIdx.z;
   if (range >= ranges) return;
@@ -285,7 +293,7 @@ attn_decode_kernel(const AttnDecodeArgs p) {
   u32x4 qf[KW];
   float qs[NG], qb[NG];
   {
-    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.ldq + (int64_t)(head0 + min(r, nh - 1)) * D;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)b * p.ldq + (int64_t)(head0 + min(hr, nh - 1)) * D;
 #pragma unroll
     for (int g = 0; g < NG; ++g) qs[g] = qb[g] = 0.0f;
 #pragma unroll
@@ -294,7 +302,7 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       __builtin_memcpy(e, __builtin_assume_aligned(src + 32 * s + 8 * q, 16), 16);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        f[i] = r < nh ? e[kCodeOrder[i]] : (T)0.0f;
+        f[i] = hr < nh ? e[kCodeOrder[i]] : (T)0.0f;
         qs[s / SG] += (float)f[i];
         qb[s / SG] += code_bias<T>(i) * (float)f[i];
       }
@@ -363,74 +371,98 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       __builtin_memcpy(__builtin_assume_aligned(&spread_v[wave][0][(lane & 31) * NG], 4 * NG), sc, 4 * NG);
       __builtin_memcpy(__builtin_assume_aligned(&spread_v[wave][1][(lane & 31) * NG], 4 * NG), mid, 4 * NG);
     }
-    uint32_t kp[2][4 * NG];
-    float vs[2][4 * NG], vm[2][4 * NG];
+    const int tile0 = P == 2 ? half : 0;   // of the lane's first values
+    uint32_t kp[VS][4 * NG];
+    float vs[VS][4 * NG], vm[VS][4 * NG];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      __builtin_memcpy(kp[t], __builtin_assume_aligned(&spread_k[wave][(16 * t + 4 * q) * NG], 16), 16 * NG);
-      __builtin_memcpy(vs[t], __builtin_assume_aligned(&spread_v[wave][0][(16 * t + 4 * q) * NG], 16), 16 * NG);
-      __builtin_memcpy(vm[t], __builtin_assume_aligned(&spread_v[wave][1][(16 * t + 4 * q) * NG], 16), 16 * NG);
+    for (int u = 0; u < VS; ++u) {
+      const int at = (16 * (tile0 + u) + 4 * q) * NG;
+      __builtin_memcpy(kp[u], __builtin_assume_aligned(&spread_k[wave][at], 16), 16 * NG);
+      __builtin_memcpy(vs[u], __builtin_assume_aligned(&spread_v[wave][0][at], 16), 16 * NG);
+      __builtin_memcpy(vm[u], __builtin_assume_aligned(&spread_v[wave][1][at], 16), 16 * NG);
     }
-    float s[2][4];
+    float s[VS][4];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int u = 0; u < VS; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[t][j] = 0.0f;
+      for (int j = 0; j < 4; ++j) s[u][j] = 0.0f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        f32x4 raw = f32x4{-qb[g], -qb[g], -qb[g], -qb[g]};
+    for (int g = 0; g < NG; ++g) {
+      f32x4 raw[2];
 #pragma unroll
-        for (int k = 0; k < SG; ++k) raw = mma16<T>(code_frag<T>(f.kw[t][g * SG + k], nibbles), qf[g * SG + k], raw);
+      for (int t = 0; t < 2; ++t) {
+        raw[t] = f32x4{-qb[g], -qb[g], -qb[g], -qb[g]};
+#pragma unroll
+        for (int k = 0; k < SG; ++k) raw[t] = mma16<T>(code_frag<T>(f.kw[t][g * SG + k], nibbles), qf[g * SG + k], raw[t]);
+      }
+#pragma unroll
+      for (int u = 0; u < VS; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t w = kp[t][j * NG + g];
-          s[t][j] = __builtin_fmaf(f16_lo(w), raw[j], s[t][j]);
-          s[t][j] = __builtin_fmaf(f16_hi(w), qs[g], s[t][j]);
+          const float x = P == 2 ? (half ? raw[1][j] : raw[0][j]) : raw[u][j];
+          const uint32_t w = kp[u][j * NG + g];
+          s[u][j] = __builtin_fmaf(f16_lo(w), x, s[u][j]);
+          s[u][j] = __builtin_fmaf(f16_hi(w), qs[g], s[u][j]);
         }
-      }
     }
     // tokens outside [lo, len), and of page entries that name no page
     if (st * 32 < lo || st * 32 + 32 > len || f.known != 3) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int u = 0; u < VS; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int token = st * 32 + 16 * t + 4 * q + j;
-          if (!(f.known >> t & 1) || token < lo || token >= len) {
-            s[t][j] = -__builtin_inff();
+          const int token = st * 32 + 16 * (tile0 + u) + 4 * q + j;
+          if (!(f.known >> (tile0 + u) & 1) || token < lo || token >= len) {
+            s[u][j] = -__builtin_inff();
 #pragma unroll
-            for (int g = 0; g < NG; ++g) vs[t][j * NG + g] = vm[t][j * NG + g] = 0.0f;   // whatever is there: 0 * it is 0
+            for (int g = 0; g < NG; ++g) vs[u][j * NG + g] = vm[u][j * NG + g] = 0.0f;   // whatever is there: 0 * it is 0
           }
         }
     }
     float m = s[0][0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) m = __builtin_fmaxf(m, s[j / 4][j % 4]);
+    for (int j = 1; j < 4 * VS; ++j) m = __builtin_fmaxf(m, s[j / 4][j % 4]);
     m = max_quarters(m);
     const float now = __builtin_fmaxf(mx, m);
     const float base = now == -__builtin_inff() ? 0.0f : now * p.c;
     const float keep = __builtin_amdgcn_exp2f(__builtin_fmaf(mx, p.c, -base));
     mx = now;
-    float pt[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) pt[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j / 4][j % 4], p.c, -base));
+    float pt[VS][4];
     l *= keep;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) l += pt[j];
+    for (int u = 0; u < VS; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pt[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], p.c, -base));
+        l += pt[u][j];
+      }
     u32x4 hi[NG], lw[NG];
     f32x4 start[NG];
+    const uint32_t first = half ? 0u : ~0u;   // P = 2: whose words are the first tile's
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       om[g] *= keep;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) om[g] = __builtin_fmaf(pt[j], vm[j / 4][(j % 4) * NG + g], om[g]);
+      for (int u = 0; u < VS; ++u) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {   // a weight's upper half, and the rest of it rounded
-        const float w0 = pt[2 * j] * vs[j / 2][(2 * j % 4) * NG + g];
-        const float w1 = pt[2 * j + 1] * vs[j / 2][(2 * j % 4 + 1) * NG + g];
-        const uint32_t u0 = __builtin_bit_cast(uint32_t, w0), u1 = __builtin_bit_cast(uint32_t, w1);
-        hi[g][j] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
-        lw[g][j] = pack2<__bf16>(w0 - __builtin_bit_cast(float, u0 & 0xffff0000u), w1 - __builtin_bit_cast(float, u1 & 0xffff0000u));
+        for (int j = 0; j < 4; ++j) om[g] = __builtin_fmaf(pt[u][j], vm[u][j * NG + g], om[g]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {   // a weight's upper half, and the rest of it rounded
+          const float w0 = pt[u][2 * j] * vs[u][2 * j * NG + g], w1 = pt[u][2 * j + 1] * vs[u][(2 * j + 1) * NG + g];
+          const uint32_t u0 = __builtin_bit_cast(uint32_t, w0), u1 = __builtin_bit_cast(uint32_t, w1);
+          const uint32_t h = __builtin_amdgcn_perm(u1, u0, 0x07060302u);
+          const float r0 = w0 - __builtin_bit_cast(float, u0 & 0xffff0000u), r1 = w1 - __builtin_bit_cast(float, u1 & 0xffff0000u);
+          const uint32_t w = pack2<__bf16>(r0, r1);
+          if constexpr (P == 2) {
+            hi[g][j] = h & first;
+            hi[g][2 + j] = h & ~first;
+            lw[g][j] = w & first;
+            lw[g][2 + j] = w & ~first;
+          } else {
+            hi[g][2 * u + j] = h;
+            lw[g][2 * u + j] = w;
+          }
+        }
       }
       start[g] = mma16<__bf16>(middle, lw[g], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
       start[g] = mma16<__bf16>(middle, hi[g], start[g]);
@@ -488,14 +520,15 @@ attn_decode_kernel(const AttnDecodeArgs p) {
     const int h = idx / D, ch = idx % D;
     float m = red_m[0][h];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) m = __builtin_fmaxf(m, red_m[w][h]);
+    for (int w = 1; w < NW * P; ++w) m = __builtin_fmaxf(m, red_m[w / P][h + HC * (w % P)]);
     const float base = m == -__builtin_inff() ? 0.0f : m * p.c;
     float total_l = 0.0f, acc = 0.0f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(red_m[w][h], p.c, -base));
-      total_l += f * red_l[w][h];
-      acc += f * red[w][h][ch];
+    for (int w = 0; w < NW * P; ++w) {
+      const int col = h + HC * (w % P);
+      const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(red_m[w / P][col], p.c, -base));
+      total_l += f * red_l[w / P][col];
+      acc += f * red[w / P][col][ch];
     }
     if (ranges == 1) {
       out[h * D + ch] = (T)(total_l == 0.0f ? 0.0f : acc / total_l);   // no token: zeros
@@ -571,13 +604,17 @@ void decode_plan(int64_t batch, int kv, int g, int64_t longest, bool split, int*
   *ranges = (int)((steps + *chunk - 1) / *chunk);
 }
 
+template <class T, int D, int NG> static void decode_g(const AttnDecodeArgs& p, const dim3& grid, hipStream_t st) {
+  if (p.g <= 8) hipLaunchKernelGGL((attn_decode_kernel<T, D, NG, 2>), grid, dim3(64 * kDecodeWaves), 0, st, p);
+  else hipLaunchKernelGGL((attn_decode_kernel<T, D, NG, 1>), grid, dim3(64 * kDecodeWaves), 0, st, p);
+}
 template <class T, int D> static hipError_t decode_d(int group, const AttnDecodeArgs& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.kv * ((p.g + 15) / 16)), (unsigned)p.batch, (unsigned)p.ranges), block(64 * kDecodeWaves);
+  const dim3 grid((unsigned)(p.kv * ((p.g + 15) / 16)), (unsigned)p.batch, (unsigned)p.ranges);
   switch (D / group) {
-    case 1: hipLaunchKernelGGL((attn_decode_kernel<T, D, 1>), grid, block, 0, st, p); break;
-    case 2: hipLaunchKernelGGL((attn_decode_kernel<T, D, 2>), grid, block, 0, st, p); break;
+    case 1: decode_g<T, D, 1>(p, grid, st); break;
+    case 2: decode_g<T, D, 2>(p, grid, st); break;
     case 4:
-      if constexpr (D == 128) { hipLaunchKernelGGL((attn_decode_kernel<T, D, 4>), grid, block, 0, st, p); break; }
+      if constexpr (D == 128) { decode_g<T, D, 4>(p, grid, st); break; }
       [[fallthrough]];
     default: return hipErrorInvalidValue;
   }
