@@ -213,8 +213,8 @@ hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t 
 // The weights are split in two bf16 parts (16 bits together, f32's range: no
 // scale of the values can make them underflow).
 //
-// A block has the up to 16 query heads of one key head and one range of the
-// sequence; its waves take steps of 32 tokens, the next step's codes in flight
+// A block has the up to 16 query heads of one key head and a piece of the
+// sequence, or several of both; its waves take steps of 32 tokens, the next step's codes in flight
 // under the present one's sums (three steps ahead cost registers and gained
 // nothing) and page entries 32 steps ahead.  A
 // step's scales and minima are loaded once, a word or more a lane, and spread
@@ -228,51 +228,92 @@ hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t 
 // four tokens instead of eight; the columns of the other tile get no weight,
 // and each column keeps a maximum and sums of its own until the end.
 //
-// Ranges of one sequence leave their maxima, sums and weighted values in `part`;
-// a second launch adds them in order.  (Counting the blocks and letting the
-// last one add saves the launch, but its fences write back and invalidate an
-// XCD's cache once a block: 355 us for a batch of 64, 76 with
-// the launch.)
+// Sequences of unequal lengths: a launch of two blocks a CU (the registers'
+// limit) cuts all steps of all sequences and key heads, laid end to end, into
+// equal pieces, wherever those end; the lengths are on the device, so each
+// block finds its own.  (A batch of 64 with 512 to 4096 tokens: 60 us; ranges
+// of one length for all, whose last blocks are those of the long sequences, 64.)  Pieces of
+// a sequence leave their maxima, sums and weighted values in `part`; a second
+// launch adds them in order.  (Counting the blocks and letting the last one add
+// saves the launch, but its fences write back and invalidate an XCD's cache
+// once a block: 355 us for that batch where the launch made it 76.)
 constexpr int kDecodeWaves = 4;
 
-// A sequence's tokens [lo, len), its steps of 32 tokens and their ranges.
-struct Span { int len, lo, begin, steps, ranges; };
+// A sequence's tokens [lo, len) and their steps of 32 tokens.
+struct Span { int len, lo, begin, steps; };
 __device__ __forceinline__ Span span_of(const AttnDecodeArgs& p, int b) {
   Span s;
   s.len = (int)max((int64_t)0, min((int64_t)p.lens[b], (int64_t)p.width * p.tpp * 16));
   s.lo = p.window > 0 ? max(0, s.len - p.window) : 0;
   s.begin = s.lo / 32;
   s.steps = (s.len + 31) / 32 - s.begin;
-  s.ranges = max(1, (s.steps + p.chunk - 1) / p.chunk);
   return s;
 }
 
+// The launch's positions: of every sequence, for each of its `groups` (head
+// block, key head), kPieceCost that stand for what a piece costs however short
+// it is, then its steps.  Block i has positions [i * per, (i + 1) * per).
+constexpr int kPieceCost = 8, kLeastPiece = 32;
+struct Layout { int64_t total, per, start; };   // start: of sequence b (if b < batch)
+// One wave (all lanes) adds up the sequences; `pos` >= 0: b becomes the sequence that holds it.
+__device__ __forceinline__ Layout layout_of(const AttnDecodeArgs& p, int groups, int64_t pos, int& b) {
+  const int lane = threadIdx.x & 63;
+  Layout s{0, 0, 0};
+  const int want = b;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    const int64_t v = b0 + lane < p.batch ? (int64_t)groups * (span_of(p, b0 + lane).steps + kPieceCost) : 0;
+    int64_t sum = v;   // inclusive
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      const int64_t other = __shfl_up(sum, i, 64);
+      if (lane >= i) sum += other;
+    }
+    if (pos >= 0) {
+      const uint64_t after = __ballot(v > 0 && s.total + sum > pos);   // sequences that end behind pos
+      if (after && s.total <= pos) {
+        const int at = __ffsll((unsigned long long)after) - 1;
+        b = b0 + at;
+        s.start = s.total + __shfl(sum - v, at, 64);
+      }
+    } else if (want >= b0 && want < b0 + 64) {
+      s.start = s.total + __shfl(sum - v, want - b0, 64);
+    }
+    s.total += __shfl(sum, 63, 64);
+  }
+  s.per = max((s.total + p.blocks - 1) / p.blocks, (int64_t)kLeastPiece);
+  return s;
+}
+
+template <int D, int NG> struct DecodeShared {
+  float red[kDecodeWaves][16][D + 4];
+  float red_m[kDecodeWaves][16], red_l[kDecodeWaves][16];
+  // of a wave's step, [token][group]: the keys' pairs, the values' scales and middles (of code 8)
+  __align__(16) uint32_t spread_k[kDecodeWaves][32 * NG];
+  __align__(16) float spread_v[kDecodeWaves][2][32 * NG];
+};
+
+// Steps [x, y) of sequence b for group c; part: where they go if they are not all of it (null: the output).
 template <class T, int D, int NG, int P>
-__global__ void __launch_bounds__(64 * kDecodeWaves, NG == 4 && P == 1 ? 1 : 2)
-attn_decode_kernel(const AttnDecodeArgs p) {
+__device__ __forceinline__ void decode_piece(const AttnDecodeArgs& p, DecodeShared<D, NG>& sh, int b, int c, const Span& span,
+                                             int x, int y, float* part) {
   constexpr int NW = kDecodeWaves;
   constexpr int KW = D / 32;   // steps of 32 channels
   constexpr int CI = D / 16;   // channels of a value column
   constexpr int SG = KW / NG;  // steps a group
-  constexpr int RS = D + 4;
   constexpr int HC = 16 / P;   // heads of the columns
   constexpr int VS = 2 / P;    // tiles of a lane's columns
-  __shared__ float red[NW][16][RS];
-  __shared__ float red_m[NW][16], red_l[NW][16];
-  // of a wave's step, [token][group]: the keys' pairs, the values' scales and middles (of code 8)
-  __shared__ __align__(16) uint32_t spread_k[NW][32 * NG];
-  __shared__ __align__(16) float spread_v[NW][2][32 * NG];
+  auto& red = sh.red;
+  auto& red_m = sh.red_m;
+  auto& red_l = sh.red_l;
+  auto& spread_k = sh.spread_k;
+  auto& spread_v = sh.spread_v;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
-  const int b = blockIdx.y, kvh = blockIdx.x % p.kv, hb = blockIdx.x / p.kv;
+  const int kvh = c % p.kv, hb = c / p.kv;
   const int nh = min(HC, p.g - hb * HC);   // query heads of this block
   const int head0 = kvh * p.g + hb * HC;
   const int hr = r % HC, half = r / HC;    // this lane's head, and tile if P = 2
-  const Span span = span_of(p, b);
-  const int len = span.len, lo = span.lo, ranges = span.ranges, range = blockIdx.z;
-  if (range >= ranges) return;
-  // this block's range: steps of 32 tokens from `first` on
-  const int first = span.begin + range * p.chunk, steps = min(p.chunk, span.steps - range * p.chunk);
+  const int len = span.len, lo = span.lo, first = span.begin + x, steps = y - x;
   const int mine = steps > wave ? (steps - wave + NW - 1) / NW : 0;   // this wave's: first + wave + NW i
   const int32_t* table = p.table + (int64_t)b * p.width;
   const int last_tile = len > 0 ? (len - 1) / 16 : 0;
@@ -399,9 +440,9 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       for (int u = 0; u < VS; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float x = P == 2 ? (half ? raw[1][j] : raw[0][j]) : raw[u][j];
+          const float v = P == 2 ? (half ? raw[1][j] : raw[0][j]) : raw[u][j];
           const uint32_t w = kp[u][j * NG + g];
-          s[u][j] = __builtin_fmaf(f16_lo(w), x, s[u][j]);
+          s[u][j] = __builtin_fmaf(f16_lo(w), v, s[u][j]);
           s[u][j] = __builtin_fmaf(f16_hi(w), qs[g], s[u][j]);
         }
     }
@@ -438,7 +479,7 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       }
     u32x4 hi[NG], lw[NG];
     f32x4 start[NG];
-    const uint32_t first = half ? 0u : ~0u;   // P = 2: whose words are the first tile's
+    const uint32_t front = half ? 0u : ~0u;   // P = 2: whose words are the first tile's
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       om[g] *= keep;
@@ -454,10 +495,10 @@ attn_decode_kernel(const AttnDecodeArgs p) {
           const float r0 = w0 - __builtin_bit_cast(float, u0 & 0xffff0000u), r1 = w1 - __builtin_bit_cast(float, u1 & 0xffff0000u);
           const uint32_t w = pack2<__bf16>(r0, r1);
           if constexpr (P == 2) {
-            hi[g][j] = h & first;
-            hi[g][2 + j] = h & ~first;
-            lw[g][j] = w & first;
-            lw[g][2 + j] = w & ~first;
+            hi[g][j] = h & front;
+            hi[g][2 + j] = h & ~front;
+            lw[g][j] = w & front;
+            lw[g][2 + j] = w & ~front;
           } else {
             hi[g][2 * u + j] = h;
             lw[g][2 * u + j] = w;
@@ -469,18 +510,18 @@ attn_decode_kernel(const AttnDecodeArgs p) {
     }
 #pragma unroll
     for (int i = 0; i < CI; ++i) {
-      u32x4 c;
+      u32x4 vf;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {   // tokens 2 j, 2 j + 1 of the eight
-        uint32_t x;
+        uint32_t w;
         if constexpr (D == 128)
-          x = __builtin_amdgcn_perm(f.vw[j / 2][2 * j % 4 + 1], f.vw[j / 2][2 * j % 4], i < 4 ? 0x05040100u : 0x07060302u);
+          w = __builtin_amdgcn_perm(f.vw[j / 2][2 * j % 4 + 1], f.vw[j / 2][2 * j % 4], i < 4 ? 0x05040100u : 0x07060302u);
         else
-          x = f.vw[j / 2][j % 2];
-        c[j] = ((x >> (4 * (i % 4))) & nibbles) | 0x43004300u;
+          w = f.vw[j / 2][j % 2];
+        vf[j] = ((w >> (4 * (i % 4))) & nibbles) | 0x43004300u;
       }
       const int g = i * NG / CI;
-      const f32x4 add = mma16<__bf16>(c, hi[g], mma16<__bf16>(c, lw[g], start[g]));
+      const f32x4 add = mma16<__bf16>(vf, hi[g], mma16<__bf16>(vf, lw[g], start[g]));
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = __builtin_fmaf(o[i][j], keep, add[j]);
     }
@@ -513,8 +554,6 @@ attn_decode_kernel(const AttnDecodeArgs p) {
     red_l[wave][r] = l;
   }
   __syncthreads();
-  const int64_t group = (int64_t)b * gridDim.x + blockIdx.x;   // (b, head block, key head)
-  float* part = p.part + group * p.ranges * (16 * (D + 2));   // [range][head][value, maximum, sum]
   T* out = static_cast<T*>(p.out) + (int64_t)b * p.ldo + (int64_t)head0 * D;
   for (int idx = threadIdx.x; idx < nh * D; idx += 64 * NW) {
     const int h = idx / D, ch = idx % D;
@@ -530,10 +569,10 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       total_l += f * red_l[w / P][col];
       acc += f * red[w / P][col][ch];
     }
-    if (ranges == 1) {
+    if (!part) {
       out[h * D + ch] = (T)(total_l == 0.0f ? 0.0f : acc / total_l);   // no token: zeros
     } else {
-      float* to = part + (int64_t)(range * 16 + h) * (D + 2);
+      float* to = part + h * (D + 2);   // value, maximum, sum
       to[ch] = acc;
       if (ch == 0) {
         to[D] = m;
@@ -541,26 +580,82 @@ attn_decode_kernel(const AttnDecodeArgs p) {
       }
     }
   }
+  __syncthreads();   // the next piece's waves write `red`
 }
 
-// A block adds the ranges of one head; the factors of all ranges first, then
-// 256 / D threads a channel, each a run of ranges, whose sums are added in order.
+template <class T, int D, int NG, int P>
+__global__ void __launch_bounds__(64 * kDecodeWaves, NG == 4 && P == 1 ? 1 : 2)
+attn_decode_kernel(const AttnDecodeArgs p) {
+  __shared__ DecodeShared<D, NG> sh;
+  const int groups = p.kv * ((p.g + 15) / 16);
+  int64_t pos, end, start = 0;
+  int b;
+  if (p.blocks == 0) {   // a block for each sequence and group
+    b = blockIdx.x / groups;
+    pos = blockIdx.x % groups;
+    end = pos + 1;
+  } else {
+    b = 0;
+    const Layout s = layout_of(p, groups, -1, b);
+    pos = blockIdx.x * s.per;
+    end = min(s.total, pos + s.per);
+  }
+  while (pos < end) {
+    int c = (int)pos, x = 0, y;
+    Span span;
+    if (p.blocks == 0) {
+      span = span_of(p, b);
+      y = span.steps;
+      pos = end;
+    } else {
+      start = layout_of(p, groups, pos, b).start;
+      b = __builtin_amdgcn_readfirstlane(b);
+      span = span_of(p, b);
+      const int64_t v = span.steps + kPieceCost;
+      c = (int)((pos - start) / v);
+      const int64_t at = start + c * v;
+      x = (int)max((int64_t)0, pos - at - kPieceCost);
+      y = (int)min((int64_t)span.steps, end - at - kPieceCost);
+      const bool empty = span.steps == 0 && pos == at;   // zeros, from the block with its first position
+      pos = at + v;
+      if (y <= x && !empty) continue;
+      y = max(y, 0);
+    }
+    // (the same in all lanes, which the compiler cannot see behind the shuffles)
+    c = __builtin_amdgcn_readfirstlane(c);
+    x = __builtin_amdgcn_readfirstlane(x);
+    y = __builtin_amdgcn_readfirstlane(y);
+    const bool whole = x == 0 && y == span.steps;
+    // a block has at most one piece that began before it and one that goes on behind it
+    float* part = whole ? nullptr : p.part + ((int64_t)blockIdx.x * 2 + (x > 0 ? 0 : 1)) * (16 * (D + 2));
+    decode_piece<T, D, NG, P>(p, sh, b, c, span, x, y, part);
+  }
+}
+
+// A block adds the pieces of one head; the factors of all pieces first, then
+// 256 / D threads a channel, each a run of pieces, whose sums are added in order.
 template <class T, int D>
 __global__ void __launch_bounds__(256)
 attn_decode_merge_kernel(const AttnDecodeArgs p) {
   constexpr int PARTS = 256 / D;
-  __shared__ float factor[kDecodeMaxRanges], wave_m[4], wave_l[4], sums[PARTS][D];
-  const int b = blockIdx.y, head = blockIdx.x, kvh = head / p.g, hb = (head - kvh * p.g) / 16, h = (head - kvh * p.g) % 16;
-  const Span span = span_of(p, b);
-  if (span.ranges == 1) return;   // written already
+  __shared__ float factor[kDecodeBlocks], wave_m[4], wave_l[4], sums[PARTS][D];
+  const int head = blockIdx.x, kvh = head / p.g, hb = (head - kvh * p.g) / 16, h = (head - kvh * p.g) % 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int hbs = (p.g + 15) / 16;
-  const int64_t group = ((int64_t)b * hbs + hb) * p.kv + kvh;
-  const float* part = p.part + group * p.ranges * (16 * (D + 2)) + h * (D + 2);
-  constexpr int kStride = 16 * (D + 2);   // floats between ranges
+  int b = blockIdx.y;
+  const Layout s = layout_of(p, p.kv * ((p.g + 15) / 16), -1, b);
+  const Span span = span_of(p, b);
+  const int64_t at = s.start + (hb * p.kv + kvh) * (int64_t)(span.steps + kPieceCost) + kPieceCost;   // its first step
+  const int64_t block0 = at / s.per, n64 = (at + span.steps - 1) / s.per - block0 + 1;
+  if (span.steps == 0 || n64 == 1) return;   // written already
+  const int n = (int)n64;
+  const float* part0 = p.part + h * (D + 2);
+  // piece k: of block0 + k, which it began in (k = 0) or before
+  auto piece = [&](int k) __attribute__((always_inline)) -> const float* {
+    return part0 + ((block0 + k) * 2 + (k == 0 ? 1 : 0)) * (16 * (D + 2));
+  };
   float m = -__builtin_inff();
-  for (int k = threadIdx.x; k < span.ranges; k += 256) {
-    const float v = part[(int64_t)k * kStride + D];
+  for (int k = threadIdx.x; k < n; k += 256) {
+    const float v = piece(k)[D];
     factor[k] = v;
     m = __builtin_fmaxf(m, v);
   }
@@ -570,19 +665,19 @@ attn_decode_merge_kernel(const AttnDecodeArgs p) {
   m = __builtin_fmaxf(__builtin_fmaxf(wave_m[0], wave_m[1]), __builtin_fmaxf(wave_m[2], wave_m[3]));
   const float base = m == -__builtin_inff() ? 0.0f : m * p.c;
   float l = 0.0f;
-  for (int k = threadIdx.x; k < span.ranges; k += 256) {
+  for (int k = threadIdx.x; k < n; k += 256) {
     const float f = __builtin_amdgcn_exp2f(__builtin_fmaf(factor[k], p.c, -base));
     factor[k] = f;
-    l += f * part[(int64_t)k * kStride + D + 1];
+    l += f * piece(k)[D + 1];
   }
   for (int i = 1; i < 64; i *= 2) l += __shfl_xor(l, i, 64);
   if (lane == 0) wave_l[wave] = l;
   __syncthreads();
   l = (wave_l[0] + wave_l[1]) + (wave_l[2] + wave_l[3]);
-  const int ch = threadIdx.x % D, run = threadIdx.x / D, per = (span.ranges + PARTS - 1) / PARTS;
+  const int ch = threadIdx.x % D, run = threadIdx.x / D, per = (n + PARTS - 1) / PARTS;
   float acc = 0.0f;
 #pragma unroll 8
-  for (int k = run * per; k < min(span.ranges, (run + 1) * per); ++k) acc += factor[k] * part[(int64_t)k * kStride + ch];
+  for (int k = run * per; k < min(n, (run + 1) * per); ++k) acc += factor[k] * piece(k)[ch];
   sums[run][ch] = acc;
   __syncthreads();
   if (threadIdx.x >= D) return;
@@ -591,17 +686,11 @@ attn_decode_merge_kernel(const AttnDecodeArgs p) {
   static_cast<T*>(p.out)[(int64_t)b * p.ldo + (int64_t)head * D + ch] = (T)(l == 0.0f ? 0.0f : acc / l);
 }
 
-// Ranges of the longest sequence a call may have, and steps of 32 tokens each:
-// two blocks a CU (the registers' limit) where the sequences are long enough,
-// and no range under four steps a wave, which the second launch would outweigh.
-void decode_plan(int64_t batch, int kv, int g, int64_t longest, bool split, int* ranges, int* chunk) {
-  const int64_t blocks = batch * kv * ((g + 15) / 16), steps = std::max<int64_t>(1, (longest + 31) / 32);
-  constexpr int64_t least = 4 * kDecodeWaves;
-  const int64_t n = split ? std::min<int64_t>(std::max<int64_t>(1, kDecodeBlocks / blocks), (steps + least - 1) / least) : 1;
-  static_assert(kDecodeBlocks <= kDecodeMaxRanges, "the merge holds a factor a range");
-  const int64_t per = (steps + n - 1) / n;
-  *chunk = (int)((per + kDecodeWaves - 1) / kDecodeWaves * kDecodeWaves);
-  *ranges = (int)((steps + *chunk - 1) / *chunk);
+// Blocks of equal pieces (0: a block for each sequence and key head, and no
+// second launch): not where no sequence is longer than a piece has to be, nor
+// where there are so many sequences that their blocks even out by themselves.
+int decode_blocks(int64_t batch, int kv, int g, int64_t longest) {
+  return longest <= 32 * kLeastPiece || batch * kv * ((g + 15) / 16) >= 8 * kDecodeBlocks ? 0 : kDecodeBlocks;
 }
 
 template <class T, int D, int NG> static void decode_g(const AttnDecodeArgs& p, const dim3& grid, hipStream_t st) {
@@ -609,7 +698,7 @@ template <class T, int D, int NG> static void decode_g(const AttnDecodeArgs& p, 
   else hipLaunchKernelGGL((attn_decode_kernel<T, D, NG, 1>), grid, dim3(64 * kDecodeWaves), 0, st, p);
 }
 template <class T, int D> static hipError_t decode_d(int group, const AttnDecodeArgs& p, hipStream_t st) {
-  const dim3 grid((unsigned)(p.kv * ((p.g + 15) / 16)), (unsigned)p.batch, (unsigned)p.ranges);
+  const dim3 grid(p.blocks ? (unsigned)p.blocks : (unsigned)(p.batch * p.kv * ((p.g + 15) / 16)));
   switch (D / group) {
     case 1: decode_g<T, D, 1>(p, grid, st); break;
     case 2: decode_g<T, D, 2>(p, grid, st); break;
@@ -618,8 +707,8 @@ template <class T, int D> static hipError_t decode_d(int group, const AttnDecode
       [[fallthrough]];
     default: return hipErrorInvalidValue;
   }
-  if (p.ranges > 1)
-    hipLaunchKernelGGL((attn_decode_merge_kernel<T, D>), dim3((unsigned)(p.kv * p.g), grid.y), dim3(256), 0, st, p);
+  if (p.blocks)
+    hipLaunchKernelGGL((attn_decode_merge_kernel<T, D>), dim3((unsigned)(p.kv * p.g), (unsigned)p.batch), dim3(256), 0, st, p);
   return hipGetLastError();
 }
 hipError_t run_attn_decode(int dtype, int dim, int group, const AttnDecodeArgs& p, hipStream_t st) {

@@ -2517,7 +2517,7 @@ extern "C" int ohip_attn_decode(ohip_ctx* ctx, const ohip_attn_decode_desc* d, c
   if (d->batch == 0) return OHIP_OK;
   if (!q || !lens || !out || (d->width > 0 && !table)) return fail(OHIP_E_INVALID, "ohip_attn_decode: null argument");
   const int64_t w = (int64_t)d->heads * cache->head_dim;
-  if (d->batch > 65535) return fail(OHIP_DECLINED, "ohip_attn_decode: more than 65535 sequences");
+  if (d->batch > 65535 || d->batch * d->heads > INT_MAX / 2) return fail(OHIP_DECLINED, "ohip_attn_decode: more than 65535 sequences");
   if ((int64_t)d->width * cache->page > INT_MAX - 64) return fail(OHIP_DECLINED, "ohip_attn_decode: sequences too long");
   AttnDecodeArgs p{};
   p.q = q; p.out = out; p.ldq = d->ldq ? d->ldq : w; p.ldo = d->ldo ? d->ldo : w;
@@ -2530,14 +2530,13 @@ extern "C" int ohip_attn_decode(ohip_ctx* ctx, const ohip_attn_decode_desc* d, c
   p.c = d->scale * 1.4426950408889634f;
   std::lock_guard<std::mutex> lock(ctx->mu);
   ctx->counters.dispatches++;
-  const int64_t groups = d->batch * p.kv * ((p.g + 15) / 16), longest = std::min((int64_t)d->width * cache->page, d->window > 0 ? (int64_t)d->window + 31 : INT64_MAX);
-  const size_t each = (size_t)groups * 16 * (cache->head_dim + 2) * sizeof(float);   // bytes a range
-  decode_plan(d->batch, p.kv, p.g, longest, true, &p.ranges, &p.chunk);
-  if (p.ranges > 1 && scratch_frozen(ctx, ScratchPlan::rounded(each * p.ranges)))
-    decode_plan(d->batch, p.kv, p.g, longest, false, &p.ranges, &p.chunk);
-  if (p.ranges > 1) {
+  const int64_t longest = std::min((int64_t)d->width * cache->page, d->window > 0 ? (int64_t)d->window + 31 : INT64_MAX);
+  p.blocks = decode_blocks(d->batch, p.kv, p.g, longest);
+  const size_t bytes = (size_t)p.blocks * 2 * 16 * (cache->head_dim + 2) * sizeof(float);
+  if (p.blocks && scratch_frozen(ctx, ScratchPlan::rounded(bytes))) p.blocks = 0;
+  if (p.blocks) {
     ScratchPlan plan;
-    const size_t at = plan.add(each * p.ranges);
+    const size_t at = plan.add(bytes);
     if ((rc = scratch_reserve(ctx, plan.total()))) return rc;
     p.part = static_cast<float*>(scratch_at(ctx, plan, at));
   }

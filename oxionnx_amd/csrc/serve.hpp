@@ -51,12 +51,12 @@ struct AttnDecodeArgs {
   int width, tpp;              // table entries a sequence; tiles of 16 tokens a page
   int batch, kv, g, window;
   float c;                     // softmax scale times log2(e)
-  int ranges, chunk;           // blocks of the longest sequence and key head, steps of 32 tokens each
-  float* part;                 // ranges > 1: batch * kv * ceil(g / 16) * ranges * 16 * (dim + 2)
+  int blocks;                  // of equal pieces; 0: one for each sequence, key head and 16 query heads
+  float* part;                 // blocks > 0: blocks * 2 * 16 * (dim + 2)
 };
-// The ranges for sequences of up to `longest` tokens; split: whether there may be more than one.
-constexpr int kDecodeBlocks = 512, kDecodeMaxRanges = 512;
-void decode_plan(int64_t batch, int kv, int g, int64_t longest, bool split, int* ranges, int* chunk);
+// The blocks for sequences of up to `longest` tokens.
+constexpr int kDecodeBlocks = 512;
+int decode_blocks(int64_t batch, int kv, int g, int64_t longest);
 hipError_t run_attn_decode(int dtype, int dim, int group, const AttnDecodeArgs& p, hipStream_t st);
 
 struct AttnPrefillArgs {

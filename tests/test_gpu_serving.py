@@ -288,6 +288,18 @@ def test_decode_long(ctx, lens):
         assert torch.equal(ctx.attn_decode(q.cuda(), cache, table.cuda(), dlens), got)
 
 
+@pytest.mark.parametrize("kv,g", [(1, 2), (2, 9)])
+def test_decode_many_unequal(ctx, kv, g):
+    """More sequences than a wave has lanes, of unequal lengths, some empty: pieces begin and end anywhere."""
+    lens = [(37 * i * i) % 1500 if i % 7 else 0 for i in range(150)]
+    lens[3], lens[140] = 2100, 1
+    cache = full_cache(ctx, 6, sum(-(-n // 16) for n in lens) + 1, 16, kv, 64, 32)
+    table = tables(11, lens, 16, cache.pages)
+    q = normal(12, (len(lens), kv * g, 64), torch.bfloat16)
+    got = ctx.attn_decode(q.cuda(), cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda())
+    R.close(got, R.decode(q, cache, table, lens, 0.125))
+
+
 def test_decode_peaked_and_scaled(ctx):
     """One key far above the rest (late, early), and values whose scales span the f16 range."""
     lens = [600]
