@@ -349,17 +349,84 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
 
   const int qi = qw + r;
   const float sum = sum_halves(l);
-  if (qi >= nq) return;
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;   // a row that sees no key: zeros
-  T* dst = static_cast<T*>(p.out) + (q0 + qi) * p.ldo + (int64_t)head * p.dim;
-#pragma unroll
-  for (int t = 0; t < OT; ++t)
+  T* dst = static_cast<T*>(p.out) + (q0 + min(qi, nq - 1)) * p.ldo + (int64_t)head * p.dim + 4 * h2;
+  auto store = [&](const f32x16& x, int t) __attribute__((always_inline)) {
+    if (qi >= nq) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int ch = 32 * t + 8 * i + 4 * h2;
-      const u32x2 w = {pack2<T>(o[t][4 * i] * inv, o[t][4 * i + 1] * inv), pack2<T>(o[t][4 * i + 2] * inv, o[t][4 * i + 3] * inv)};
-      if (ch < p.dim) *reinterpret_cast<u32x2*>(dst + ch) = w;
+      const u32x2 w = {pack2<T>(x[4 * i] * inv, x[4 * i + 1] * inv), pack2<T>(x[4 * i + 2] * inv, x[4 * i + 3] * inv)};
+      if (32 * t + 8 * i + 4 * h2 < p.dim) *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = w;
     }
+  };
+  float finite = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16 * OT; ++i) finite = __builtin_fmaf(o[i / 16][i % 16], 0.0f, finite);
+  if (!__any(qi < nq && finite != 0.0f)) {
+#pragma unroll
+    for (int t = 0; t < OT; ++t) store(o[t], t);
+    return;
+  }
+  // A weight of 0 times a value that is not finite is NaN: such a value of a
+  // key that a query does not see has reached its sums, if the half tile holds
+  // keys that it sees.  Such a wave takes its sums again, from memory and 32
+  // channels at a time: of the finite values, and (with ones for weights) of
+  // the infinities of either sign that each query sees; a NaN counts as both.
+  constexpr uint32_t kExp = std::is_same<T, _Float16>::value ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t kOne = std::is_same<T, _Float16>::value ? 0x3c00u : 0x3f80u;
+  const float off = base == -__builtin_inff() ? 0.0f : base;
+#pragma unroll 1
+  for (int t = 0; t < OT; ++t) {
+    f32x16 x, plus, minus;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = plus[i] = minus[i] = 0.0f;
+#pragma unroll 1
+    for (int j = 0; j < halves; ++j) {
+      const int kj = kbeg + 32 * j;
+      f32x16 a;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) a[i] = 0.0f;
+      const char* krow = kb + (int64_t)min(kj + r, nk - 1) * p.ldk * 2;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int ch = 16 * k + 8 * h2;
+        u32x4 f = {0, 0, 0, 0};
+        if (ch < p.dim) __builtin_memcpy(&f, __builtin_assume_aligned(krow + ch * 2, 16), 16);
+        a = mma32<T>(f, qf[k], a);
+      }
+      mask(j, a);
+      const int ch = 32 * t + r;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        u32x4 w, sees, v, vp, vm;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float s0 = a[8 * k + 2 * e], s1 = a[8 * k + 2 * e + 1];
+          sees[e] = (s0 == -__builtin_inff() ? 0u : kOne) | (s1 == -__builtin_inff() ? 0u : kOne << 16);
+          w[e] = pack2<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s0, p.c, -off)), __builtin_amdgcn_exp2f(__builtin_fmaf(s1, p.c, -off)));
+          v[e] = vp[e] = vm[e] = 0;
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int key = min(kj + 16 * k + 8 * (e / 2) + 4 * h2 + 2 * (e % 2) + b, nk - 1);
+            const uint32_t y = ch < p.dim ? *reinterpret_cast<const uint16_t*>(vb + ((int64_t)key * p.ldv + ch) * 2) : 0u;
+            const bool big = (y & kExp) == kExp, nan = (y & 0x7fffu) > kExp;
+            v[e] |= (big ? 0u : y) << (16 * b);
+            vp[e] |= (nan || y == kExp ? kOne : 0u) << (16 * b);
+            vm[e] |= (nan || y == (kExp | 0x8000u) ? kOne : 0u) << (16 * b);
+          }
+        }
+        x = mma32<T>(v, w, x);
+        plus = mma32<T>(vp, sees, plus);
+        minus = mma32<T>(vm, sees, minus);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[i] += plus[i] > 0.0f ? __builtin_inff() : 0.0f;
+      x[i] -= minus[i] > 0.0f ? __builtin_inff() : 0.0f;
+    }
+    store(x, t);
+  }
 }
 
 template <class T, int D, int NW> static hipError_t prefill_l(const AttnPrefillArgs& p, hipStream_t st) {

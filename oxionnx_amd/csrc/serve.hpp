@@ -104,8 +104,6 @@ template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 __device__ __forceinline__ float f16_lo(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
 __device__ __forceinline__ float f16_hi(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
 
 // Eight codes of a word as a fragment of T, each plus a bias that is exact in
 // T, elements in the order of channels 0, 4, 1, 5, 2, 6, 3, 7: a code in the

@@ -408,6 +408,42 @@ def test_prefill_sequences_do_not_meet(ctx):
     assert out[40:70].isnan().all() and (out[120:] == 5).all()
 
 
+@pytest.mark.parametrize("dtype", HALF, ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 80, 128])
+@pytest.mark.parametrize("window", [0, 20])
+def test_prefill_unseen_values(ctx, dtype, dim, window):
+    """Infinities and NaN of keys that a query does not see leave its row as it is; those that it sees reach the
+    channels they stand in."""
+    lens, ks, kv = [150, 30, 70], [150, 45, 50], 2   # the last sequence's first queries see no key
+    cu_q, cu_k = offsets(lens), offsets(ks)
+    q = normal(41, (250, kv, dim), dtype)
+    k, v = (normal(42 + i, (245, kv, dim), dtype) for i in range(2))
+    bad = [(70, 0, 3, float("nan")), (75, 0, 3, float("inf")), (100, 1, 40, float("inf")), (101, 1, 40, float("-inf")),
+           (160, 0, 11, float("-inf")), (200, 0, dim - 1, float("inf")), (200, 1, 0, float("nan"))]
+    clean = v.clone()
+    for row, head, ch, x in bad:
+        v[row, head, ch], clean[row, head, ch] = x, 0.0
+    k[145, 1, 5] = float("nan")
+    got = ctx.attn_prefill(q.cuda(), k.cuda(), v.cuda(), cu_q.cuda(), cu_k.cuda(), window=window).cpu().double()
+    k[145, 1, 5] = 0.0
+    value, bound = R.prefill(q, k, clean, cu_q, cu_k, dim ** -0.5, True, window)
+    for i in range(3):
+        for a in range(lens[i]):
+            last, row = a + ks[i] - lens[i], int(cu_q[i]) + a
+            seen = range(max(0, last - window + 1 if window else 0) + int(cu_k[i]), last + 1 + int(cu_k[i]))
+            for head in range(kv):
+                if 145 in seen and head == 1 and i == 0:
+                    assert got[row, head].isnan().all()
+                    continue
+                want = value[row, head].clone()
+                for at, h, ch, x in bad:
+                    if h == head and at in seen:
+                        want[ch] += x if abs(want[ch]) != float("inf") or x != x or x == want[ch] else float("nan")
+                plain = want.isfinite()
+                assert ((got[row, head] - want).abs() <= bound[row, head])[plain].all()
+                np.testing.assert_array_equal(got[row, head][~plain].numpy(), want[~plain].numpy())
+
+
 def test_prefill_offsets_outside(ctx):
     """Offsets beyond the tokens (and falling ones) read and write nothing outside."""
     dim = 64
