@@ -3,8 +3,8 @@
 
 namespace ohip {
 
-// A block has 32 * NW query rows of one head, 32 a wave, and walks the keys
-// they see in tiles of 64 that all its waves share through LDS.  S^T = K Q^T,
+// A block has 128 query rows of one head, 32 a wave, and walks the keys they
+// see in tiles of 64 that its four waves share through LDS.  S^T = K Q^T,
 // so a lane holds one query (its column) and the softmax's running maximum and
 // sum need one exchange between a lane and the one 32 further; O^T = V^T P^T
 // takes P as it lies in the registers: k index 8 h + j (h = lane / 32) stands
@@ -14,9 +14,15 @@ namespace ohip {
 // Bound: the matrix products, with about as many cycles of vector instructions
 // (two thirds of them the exponentials and their arguments), so each stage
 // interleaves the softmax of one half tile with the products of its
-// neighbours; and the latency of the tiles, which are loaded straight into
-// LDS three passes ahead.
-constexpr int kPrefillK = 64, kPrefillBufs = 4;
+// neighbours.  Tiles are loaded straight into LDS a pass ahead; a CU has room
+// for two blocks, each of which works through the other's barriers, its first
+// tiles and its last rows.  32 heads, 8 of keys, of 128 channels: 8192 tokens
+// 535 us (1026 TFLOP/s, 75 % of a large matrix product's rate), seven prompts
+// of 8191 tokens 141, the last 1000 of 4000 within 2048 51.  Eight waves that
+// share a tile and load three passes ahead, one block a CU: 546, 153 and 71;
+// four of them 728, 222 and 60.  Blocks in the order of their keys, most
+// first, through all sequences: 536, 141, and 0.2 us more for a short prompt.
+constexpr int kPrefillK = 64, kPrefillQ = 128;
 
 // Slot of 16-byte chunk c of a staged row r: rows of 16 (8) chunks, XOR with a
 // permutation of r's low bits that puts 16 consecutive rows of one chunk (the
@@ -28,42 +34,40 @@ template <int CH> __device__ __forceinline__ int row_swizzle(int r) {
 }
 
 // Which sequence a block's tile belongs to.  Sequence i has the tile slots
-// from cu[i] / BQ + i on (at least as many as it has tiles), so that the grid
+// from cu[i] / 128 + i on (at least as many as it has tiles), so that the grid
 // needs only the totals; a slot past its sequence's end has nothing to do.
 // One wave searches; offsets that are not ascending cannot lead outside
 // [0, total].
-__device__ __forceinline__ int slot_sequence(const int32_t* cu, int seqs, int64_t total, int tile, int bq) {
+__device__ __forceinline__ int slot_sequence(const int32_t* cu, int seqs, int64_t total, int tile) {
   const int lane = threadIdx.x & 63;
   int n = 0;
   for (int i0 = 0; i0 < seqs; i0 += 64) {
     const int i = i0 + lane;
     const int64_t c = i < seqs ? min(max((int64_t)cu[i], (int64_t)0), total) : 0;
-    n += __popcll(__ballot(i < seqs && c / bq + i <= tile));
+    n += __popcll(__ballot(i < seqs && c / kPrefillQ + i <= tile));
   }
   return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-template <class T, int D, int NW>
-__global__ void __launch_bounds__(64 * NW, 2)
+template <class T, int D>
+__global__ void __launch_bounds__(256, 2)
 attn_prefill_kernel(const AttnPrefillArgs p) {
-  constexpr int BQ = 32 * NW, BK = kPrefillK, KS = D / 16, OT = D / 32;
+  constexpr int NW = 4, BQ = kPrefillQ, BK = kPrefillK, KS = D / 16, OT = D / 32;
   constexpr int CH = D > 64 ? 16 : 8, RB = CH * 16;     // chunks and bytes of a staged row
   constexpr int NL = BK * CH / (64 * NW);               // loads a thread of a tile
-  constexpr int NB = kPrefillBufs;
   constexpr int kTile = BK * RB;
   static_assert(NL >= 1 && (64 / CH) * NW % 16 == 0, "a thread's loads share their swizzle");
   // K and V tiles, each a variable of its own: the compiler then knows which
   // loads a fragment read may depend on, and waits for no later ones
-  __shared__ __align__(256) char lk0[kTile], lk1[kTile], lk2[kTile], lk3[kTile];
-  __shared__ __align__(256) char lv0[kTile], lv1[kTile], lv2[kTile], lv3[kTile];
+  __shared__ __align__(256) char lk0[kTile], lk1[kTile], lv0[kTile], lv1[kTile];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 31, h2 = lane >> 5;
   // heads of one key head next to each other in time, key heads eight apart: an XCD's L2 holds its own
   const int kvh = blockIdx.x % p.kv, head = kvh * p.g + blockIdx.x / p.kv;
   const int tile = (int)gridDim.y - 1 - (int)blockIdx.y;   // late tiles of a sequence see the most keys
-  const int seq = slot_sequence(p.cu_q, p.seqs, p.q_tokens, tile, BQ);
+  const int seq = slot_sequence(p.cu_q, p.seqs, p.q_tokens, tile);
   if (seq < 0) return;
   const int64_t q0 = min(max((int64_t)p.cu_q[seq], (int64_t)0), p.q_tokens);
   const int64_t q1 = min(max((int64_t)p.cu_q[seq + 1], q0), p.q_tokens);
@@ -234,8 +238,8 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
     }
     softmax(cur, w);
     // In the wave's order: the fragments' loads and the maximum between the
-    // first products, then the exponentials (530 us for the 8192-token prompt;
-    // 546 in the compiler's order, 562 with all loads in front).
+    // first products, then the exponentials (3 % faster
+    // than the compiler's order, 6 % than all loads in front: 8192 tokens).
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);     // LDS reads
@@ -255,23 +259,21 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
   constexpr int kHalf = 32 * RB;
   // Pass t: scores of tile t + 1, values of tile t.  All waves go through the
   // block's passes; a wave computes while its queries see keys.  K tile i is
-  // in variable i % NB and so is V tile i: pass t may overwrite K tile t and V
-  // tile t - 1, the last ones that pass t - 1 read, with tiles t + NB and
-  // t + NB - 1, which have NB - 1 passes to arrive.
+  // in variable i % 2 and so is V tile i: pass t may overwrite K tile t and V
+  // tile t - 1, the last ones that pass t - 1 read, with tiles t + 2 and t + 1,
+  // which arrive during it.
   auto kvar = [&](auto i) __attribute__((always_inline)) -> char* {
-    constexpr int v = decltype(i)::value % NB;
-    if constexpr (v == 0) return lk0; else if constexpr (v == 1) return lk1; else if constexpr (v == 2) return lk2; else return lk3;
+    if constexpr (decltype(i)::value % 2 == 0) return lk0; else return lk1;
   };
   auto vvar = [&](auto i) __attribute__((always_inline)) -> char* {
-    constexpr int v = decltype(i)::value % NB;
-    if constexpr (v == 0) return lv0; else if constexpr (v == 1) return lv1; else if constexpr (v == 2) return lv2; else return lv3;
+    if constexpr (decltype(i)::value % 2 == 0) return lv0; else return lv1;
   };
   int t = 0;
-  auto begin = [&](auto at) __attribute__((always_inline)) {   // at: t % NB
+  auto begin = [&](auto at) __attribute__((always_inline)) {   // at: t % 2
     constexpr int m = decltype(at)::value;
-    loads_barrier<(NB - 2) * 2 * NL>();   // all but those of the last NB - 2 passes
-    load(kb, p.ldk, t + NB, kvoff, kstep, kvar(std::integral_constant<int, m>()));
-    load(vb, p.ldv, t + NB - 1, vvoff, vstep, vvar(std::integral_constant<int, m + NB - 1>()));
+    loads_barrier<0>();
+    load(kb, p.ldk, t + 2, kvoff, kstep, kvar(std::integral_constant<int, m>()));
+    load(vb, p.ldv, t + 1, vvoff, vstep, vvar(std::integral_constant<int, m + 1>()));
   };
   auto pass = [&](auto at) __attribute__((always_inline)) {
     constexpr int m = decltype(at)::value;
@@ -297,17 +299,11 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
   };
   using C0 = std::integral_constant<int, 0>;
   using C1 = std::integral_constant<int, 1>;
-  using C2 = std::integral_constant<int, 2>;
-  using C3 = std::integral_constant<int, 3>;
   if (tiles) {
     load(kb, p.ldk, 0, kvoff, kstep, lk0);
     load(vb, p.ldv, 0, vvoff, vstep, lv0);
     load(kb, p.ldk, 1, kvoff, kstep, lk1);
-    load(vb, p.ldv, 1, vvoff, vstep, lv1);
-    load(kb, p.ldk, 2, kvoff, kstep, lk2);
-    load(vb, p.ldv, 2, vvoff, vstep, lv2);
-    load(kb, p.ldk, 3, kvoff, kstep, lk3);
-    loads_barrier<6 * NL>();   // K tile 0
+    loads_barrier<2 * NL>();   // K tile 0
     if (halves > 0) {
       scores(lk0, s[0]);
       mask(0, s[0]);
@@ -315,34 +311,16 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
       softmax(s[0], pf);
     }
   }
-  while (2 * t + 8 < halves) {
+  while (2 * t + 4 < halves) {
     pass(C0());
     pass(C1());
-    pass(C2());
-    pass(C3());
   }
-  if (2 * t + 2 < halves) {
-    pass(C0());
-    if (2 * t + 2 < halves) {
-      pass(C1());
-      if (2 * t + 2 < halves) pass(C2());
-    }
-  }
+  if (2 * t + 2 < halves) pass(C0());
   if (halves > 0) {
-    switch (t % NB) {
-      case 0: last(C0()); break;
-      case 1: last(C1()); break;
-      case 2: last(C2()); break;
-      default: last(C3()); break;
-    }
+    if (t % 2 == 0) last(C0()); else last(C1());
   }
   while (t < tiles) {
-    switch (t % NB) {
-      case 0: begin(C0()); break;
-      case 1: begin(C1()); break;
-      case 2: begin(C2()); break;
-      default: begin(C3()); break;
-    }
+    if (t % 2 == 0) begin(C0()); else begin(C1());
     ++t;
   }
   loads_barrier<0>();   // those of tiles past the end write LDS too
@@ -429,18 +407,10 @@ attn_prefill_kernel(const AttnPrefillArgs p) {
   }
 }
 
-template <class T, int D, int NW> static hipError_t prefill_l(const AttnPrefillArgs& p, hipStream_t st) {
-  constexpr int BQ = 32 * NW;
-  hipLaunchKernelGGL((attn_prefill_kernel<T, D, NW>), dim3((unsigned)(p.kv * p.g), (unsigned)(p.q_tokens / BQ + p.seqs)),
-                     dim3(64 * NW), 0, st, p);
-  return hipGetLastError();
-}
 template <class T, int D> static hipError_t prefill_d(const AttnPrefillArgs& p, hipStream_t st) {
-  // Eight waves (256 queries) share each tile of keys; where that leaves CUs
-  // without a block, four: 1000 queries x 32 heads of 3000-4000 keys 58 us
-  // against 71, 8192 x 32 728 against 530.
-  const int64_t wide = (int64_t)p.kv * p.g * (p.q_tokens / 256 + p.seqs);
-  return wide < 256 ? prefill_l<T, D, 4>(p, st) : prefill_l<T, D, 8>(p, st);
+  hipLaunchKernelGGL((attn_prefill_kernel<T, D>), dim3((unsigned)(p.kv * p.g), (unsigned)(p.q_tokens / kPrefillQ + p.seqs)),
+                     dim3(256), 0, st, p);
+  return hipGetLastError();
 }
 template <class T> static hipError_t prefill_t(const AttnPrefillArgs& p, hipStream_t st) {
   if (p.dim <= 64) return prefill_d<T, 64>(p, st);
