@@ -123,19 +123,36 @@ template <> struct Q4Mma<float> {
   }
 };
 
+// Slots of 128 k of activations that a wave has in LDS: four waves a block
+// leave room for four blocks a CU (16 x 4096 x 11008 bf16 9.3 us, two blocks
+// with twice the slots 11.0), eight are alone on theirs.
+template <class T, int TM, int NW> constexpr int q4_slots() {
+  constexpr int n = ((NW == 4 ? 32 : 128) << 10) / (NW * 16 * TM * 128 * (int)sizeof(T));
+  return n >= 4 ? 4 : n;
+}
+
 // A block takes 16 rows of the weight; its NW waves split K and meet in LDS in
 // wave order.  GS: steps of 32 k a group holds (four for any larger).
-// Bound: streaming the weight once, and for more rows the activations' traffic
-// from L2 (M * K elements a block).  Both need loads in flight: a ring of
-// tiles of 128 k of codes, and the next tile's activations.
-template <class T, int TM, int GS, int NW>
+// Bound: streaming the weight once, and the lookups of the activations in the
+// CU's cache: a fragment's neighbouring lanes are of different rows, so a load
+// of it is 64 lookups of 16 bytes.  STAGE copies them into LDS instead, 64
+// bytes a lookup, and reads the fragments there (16 x 11008 x 4096 bf16 14.5 ->
+// 9.8 us, 64 rows 46 -> 21).  A ring of tiles of 128 k of codes and of
+// activations is in flight.
+template <class T, int TM, int GS, int NW, bool STAGE>
 __global__ void __launch_bounds__(64 * NW, NW / 4)
 q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes, const T* __restrict__ scales,
           const uint8_t* __restrict__ zp, int M, int N, int K, int group, const FloatEpi<T> epi) {
   __shared__ f32x4 red[NW][TM][64];
   constexpr int GN = 4 / GS;   // groups of a tile
-  // (what the registers hold: a tile of activations is 8 TM registers of f16, 16 of f32)
+  // (what the registers hold: a tile of activations is 16 TM registers of f16, 32 of f32)
   constexpr int kRing = TM * sizeof(T) <= 4 ? 4 : 2, kActs = TM * sizeof(T) <= 4 ? 2 : 1;
+  // staged: slots of 16 TM rows, chunk c of row r in place c ^ r % 16
+  constexpr int kChunks = 8 * sizeof(T), kSlot = 16 * TM * kChunks * 16, kSlots = q4_slots<T, TM, NW>();
+  constexpr int kStage = 16 * TM * kChunks / 64;   // loads of a tile's activations
+  static_assert(!STAGE || (kSlots >= 1 && kRing % kSlots == 0 && (kSlots - 1) * kStage + kSlots * (1 + GN) < 64), "");
+  __shared__ __align__(256) char st0[STAGE ? NW * kSlot : 16], st1[STAGE && kSlots > 1 ? NW * kSlot : 16];
+  __shared__ __align__(256) char st2[STAGE && kSlots > 2 ? NW * kSlot : 16], st3[STAGE && kSlots > 2 ? NW * kSlot : 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int shift = GS == 1 ? 5 : GS == 2 ? 6 : group == 256 ? 8 : 7;   // log2(group)
@@ -186,7 +203,43 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
         }
     }
   };
-  auto sum = [&](const Tile& f, const Acts& x) __attribute__((always_inline)) {
+  auto slot = [&](int i) __attribute__((always_inline)) -> char* {
+    const int v = i % kSlots;
+    return (v == 0 ? st0 : v == 1 ? st1 : v == 2 ? st2 : st3) + wave * kSlot;
+  };
+  const auto rs = rows_resource(reinterpret_cast<const char*>(a), (int)(((M - 1) * lda + K) * sizeof(T)));
+  const int srow = lane / kChunks, splace = lane % kChunks;
+  auto stage = [&](int k, int i) __attribute__((always_inline)) {   // tile i into slot k
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was read there has arrived
+    char* to = slot(k);
+    const int k0 = (t0 + i) * 128;
+#pragma unroll
+    for (int j = 0; j < kStage; ++j) {
+      constexpr int kRows = 64 / kChunks;
+      const int row = j * kRows + srow, at = k0 + (splace ^ (row & 15)) * (int)(16 / sizeof(T));
+      const int off = at < K && row < M ? (int)((row * lda + at) * sizeof(T)) : (int)0x80000000u;   // else zeros
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(to + j * 1024), 16, off, 0, 0, 0);
+    }
+    asm volatile("" ::: "memory");   // the tile's other loads come after these
+  };
+  // The activations of the present tile are in LDS: after their loads the
+  // wave has issued at least kSlots - 1 tiles' more, and kSlots times a tile's
+  // codes and scales, unless these are the last tiles.
+  auto arrived = [&](bool more) __attribute__((always_inline)) {
+    if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kSlots - 1) * kStage + kSlots * (1 + GN)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+  auto staged = [&](int k, int s, int t) __attribute__((always_inline)) {
+    const char* row = slot(k) + (16 * t + r) * (kChunks * 16);
+    Act<T> x;
+    constexpr int kPer = sizeof(T) / 2;   // chunks of eight elements
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      __builtin_memcpy(reinterpret_cast<char*>(&x) + 16 * j,
+                       __builtin_assume_aligned(row + (((kPer * (4 * s + q) + j) ^ r) * 16), 16), 16);
+    return x;
+  };
+  auto sum = [&](const Tile& f, auto act) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < GN; ++g) {
       Q4Mma<T> mul;
@@ -198,7 +251,7 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
       for (int s = 0; s < GS; ++s) {
         const auto c = mul.frag(f.w[g * GS + s]);
 #pragma unroll
-        for (int t = 0; t < TM; ++t) raw[t] = mul.mma(c, x.x[g * GS + s][t], raw[t]);
+        for (int t = 0; t < TM; ++t) raw[t] = mul.mma(c, act(g * GS + s, t), raw[t]);
       }
 #pragma unroll
       for (int t = 0; t < TM; ++t)
@@ -208,7 +261,13 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
   };
   Tile ring[kRing];
   Acts acts[kActs];
-  if (kActs > 1 && mine > 0) load_acts(acts[0], 0);
+  if (STAGE) {
+#pragma unroll
+    for (int i = 0; i < kSlots - 1; ++i)
+      if (i < mine) stage(i, i);
+  } else if (kActs > 1 && mine > 0) {
+    load_acts(acts[0], 0);
+  }
 #pragma unroll
   for (int i = 0; i < kRing - 1; ++i)
     if (i < mine) load(ring[i], i);
@@ -217,9 +276,15 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
     for (int k = 0; k < kRing; ++k) {
       if (i + k >= mine) break;
       // (the activations first: loads arrive in order, and these are waited for next)
-      if (i + k + kActs - 1 < mine) load_acts(acts[(k + kActs - 1) % kActs], i + k + kActs - 1);
+      if (STAGE) {
+        if (i + k + kSlots - 1 < mine) stage(k + kSlots - 1, i + k + kSlots - 1);
+      } else if (i + k + kActs - 1 < mine) {
+        load_acts(acts[(k + kActs - 1) % kActs], i + k + kActs - 1);
+      }
       if (i + k + kRing - 1 < mine) load(ring[(k + kRing - 1) % kRing], i + k + kRing - 1);
-      sum(ring[k], acts[k % kActs]);
+      if constexpr (STAGE) arrived(i + k + kRing - 1 < mine);
+      if constexpr (STAGE) sum(ring[k], [&](int s, int t) __attribute__((always_inline)) { return staged(k, s, t); });
+      else sum(ring[k], [&](int s, int t) __attribute__((always_inline)) { return acts[k % kActs].x[s][t]; });
     }
   }
 #pragma unroll
@@ -241,28 +306,38 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
   store_group(out, epi.out_bytes(), out.row(i), i, j, bits);
 }
 
-template <class T, int TM, int NW>
+template <class T, int TM, int NW, bool STAGE>
 static hipError_t q4_w(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
   const T* a = static_cast<const T*>(g.a);
   const u32x4* codes = static_cast<const u32x4*>(g.codes);
   const T* sc = static_cast<const T*>(g.scales);
   const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * NW);
   if (g.group == 32)
-    hipLaunchKernelGGL((q4_kernel<T, TM, 1, NW>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 1, NW, STAGE>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
   else if (g.group == 64)
-    hipLaunchKernelGGL((q4_kernel<T, TM, 2, NW>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 2, NW, STAGE>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
   else
-    hipLaunchKernelGGL((q4_kernel<T, TM, 4, NW>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 4, NW, STAGE>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
   return hipGetLastError();
 }
-// Four waves a block where there are two blocks a CU, which then hold all of
-// the launch at once (1 x 4096 x 11008 f16, 688 blocks: 8.9 us, eight waves
-// 9.5); else eight (16 x 11008 x 4096 bf16, 256 blocks: 14.8, four 17.5,
-// sixteen 14.9).
+template <class T, int TM, int NW> static hipError_t q4_s(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
+  if constexpr (q4_slots<T, TM, NW>() > 0) {
+    const int64_t bytes = ((g.M - 1) * g.lda + g.K) * (int64_t)sizeof(T);
+    // Whole aligned chunks, which 32 bits address; of fewer rows most of a
+    // slot is filled for nothing (1 x 4096 x 11008 bf16 8.4 us, staged 9.1; 4
+    // rows 9.2 and 8.8; f32 4 rows 23.6 and 25.3, 8 rows 25.4 and 25.3).
+    if (g.M > (sizeof(T) == 4 ? 4 : 2) && g.K * sizeof(T) % 16 == 0 && g.lda * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && bytes < INT_MAX)
+      return q4_w<T, TM, NW, true>(g, epi, st);
+  }
+  return q4_w<T, TM, NW, false>(g, epi, st);
+}
+// Four waves a block where there are two blocks a CU or more (1 x 4096 x 11008
+// bf16, 688 blocks, not staged: 8.4 us, eight waves 9.5; 32 rows 12.8 and 16.4), else
+// eight (16 x 11008 x 4096, 256 blocks, not staged: 14.8, four 17.5).
 template <class T, int TM> static hipError_t q4_t(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
   if constexpr (TM * sizeof(T) <= 4)
-    if (g.N >= 512 * 16) return q4_w<T, TM, 4>(g, epi, st);
-  return q4_w<T, TM, 8>(g, epi, st);
+    if (g.N >= 512 * 16) return q4_s<T, TM, 4>(g, epi, st);
+  return q4_s<T, TM, 8>(g, epi, st);
 }
 
 template <class T> static hipError_t q4_m(const Q4Args& g, const FloatOut& o, hipStream_t st) {

@@ -79,6 +79,21 @@ def test_q4_strides_and_activation(ctx, dtype, m):
     assert (out[:, 0] == 7).all() and (out[:, 1 + n:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32] + HALF, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("zp", [False, True])
+@pytest.mark.parametrize("m,k,n,group", [(58, 160, 320, 32), (16, 224, 160, 32), (30, 4104, 8200, 128), (3, 2600, 8192, 64),
+                                         (64, 11008, 48, 256), (20, 136, 33, 64)])
+def test_q4_aligned_rows(ctx, dtype, zp, m, k, n, group):
+    """Rows of whole 16-byte chunks, a last tile of any length, two weights in turn."""
+    cases = [q4_case(m + i, m, k, n, group, zp, dtype) for i in range(2)]
+    ws = [q4_weight(ctx, codes, scales, zeros, k) for _, codes, scales, zeros, _ in cases]
+    dev = [c[0].cuda() for c in cases]
+    outs = [ctx.gemm_q4(dev[i % 2], ws[i % 2]) for i in range(4)]
+    assert (outs[0] == outs[2]).all() and (outs[1] == outs[3]).all()
+    for (a, codes, scales, zeros, _), got in zip(cases, outs):
+        R.close(got, R.gemm_q4(a, codes, scales, zeros))
+
+
 def test_q4_infinite_row_stays_in_its_row(ctx):
     a, codes, scales, zeros, bias = q4_case(4, 4, 256, 32, 32, True, torch.float16)
     a[2, 7] = float("nan")
