@@ -215,13 +215,14 @@ hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t 
 //
 // A block has the up to 16 query heads of one key head and a piece of the
 // sequence, or several of both; its waves take steps of 32 tokens, the next
-// step's codes in flight under the present one's sums (three steps ahead cost
-// registers and gained nothing) and page entries 32 steps ahead.  A step's
-// scales and minima are loaded once, a word or more a lane, and spread to the
-// lanes that need them through LDS.  S^T = K Q^T, lane l = 16 q + h: head h,
-// tokens 4 q + r of two tiles of 16, which is how O^T = V^T P^T wants its right
-// operand when the values' tokens are counted 4 q + j of the first tile, then
-// of the second.
+// step's codes in flight under the present one's sums (the batch below: three
+// steps 56 us, two 54.6) and page entries 32 steps ahead.  The last step loads
+// once more what it has: a load that only some steps issue would make all of
+// them wait for it (60 us).  A step's scales and minima are loaded once, a word
+// or more a lane, and spread to the lanes that need them through LDS.
+// S^T = K Q^T, lane l = 16 q + h: head h, tokens 4 q + r of two tiles of 16,
+// which is how O^T = V^T P^T wants its right operand when the values' tokens
+// are counted 4 q + j of the first tile, then of the second.
 //
 // Up to eight heads leave half of the sixteen columns free: then (P = 2) a
 // column is a head of one of the two tiles, so that a lane has the softmax of
@@ -231,17 +232,18 @@ hipError_t run_kv_append(int dtype, int dim, const KvAppendArgs& p, hipStream_t 
 // Sequences of unequal lengths: a launch of two blocks a CU (the registers'
 // limit) cuts all steps of all sequences and key heads, laid end to end, into
 // equal pieces, wherever those end; the lengths are on the device, so each
-// block finds its own.  (A batch of 64 with 512 to 4096 tokens: 60 us; ranges
-// of one length for all, whose last blocks are those of the long sequences,
-// 64.)  Pieces of a sequence leave their maxima, sums and weighted values in
+// block finds its own.  (A batch of 64 with 512 to 4096 tokens: 7 % less time
+// than ranges of one length for all, whose last blocks are those of the long
+// sequences.)  Pieces of a sequence leave their maxima, sums and weighted values in
 // `part`; a second launch adds them in order.  (Counting the blocks and letting
 // the last one add saves the launch, but its fences write back and invalidate
 // an XCD's cache once a block: 355 us for that batch where the launch made it
 // 76.)
 //
 // Bound: the latency of a step with two waves a SIMD, for which the registers
-// allow no third (that batch: 51 us and 7 of the second launch; its loads
-// alone 38; two sequences of 131071 and 73728 tokens 63, 53 and 6, 47).
+// allow no third (that batch: 54.6 us, 7 of them the second launch; its loads
+// alone 38; two sequences of 131071 and 73728 tokens 57.8, 6, 47).  Codes
+// copied into LDS, 64 bytes a cache lookup instead of 16: 62 us.
 constexpr int kDecodeWaves = 4;
 
 // A sequence's tokens [lo, len) and their steps of 32 tokens.
@@ -531,16 +533,13 @@ __device__ __forceinline__ void decode_piece(const AttnDecodeArgs& p, DecodeShar
       for (int j = 0; j < 4; ++j) o[i][j] = __builtin_fmaf(o[i][j], keep, add[j]);
     }
   };
-  constexpr int kRing = 2;
-  Step ring[kRing];
+  Step ring[2];
+  if (mine > 0) load(ring[0], 0);
+  for (int i = 0; i < mine; i += 2) {
 #pragma unroll
-  for (int i = 0; i < kRing - 1; ++i)
-    if (i < mine) load(ring[i], i);
-  for (int i = 0; i < mine; i += kRing) {
-#pragma unroll
-    for (int k = 0; k < kRing; ++k) {
+    for (int k = 0; k < 2; ++k) {
       if (i + k >= mine) break;
-      if (i + k + kRing - 1 < mine) load(ring[(k + kRing - 1) % kRing], i + k + kRing - 1);
+      load(ring[1 - k], min(i + k + 1, mine - 1));
       sum(ring[k], i + k);
     }
   }
