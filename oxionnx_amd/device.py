@@ -141,6 +141,8 @@ class KvCache:
     @staticmethod
     def empty(pages, page, kv_heads, head_dim, group=64, device=0):
         """A cache of zeros."""
+        if min(pages, page, kv_heads, head_dim, group) <= 0 or page % 16 or head_dim % 32 or head_dim % group:
+            raise _invalid("KvCache: pages are a multiple of 16 tokens, heads of 32 channels, groups divide the head")
         torch = _torch()
         at = torch.device("cuda", device)
         params = (pages, kv_heads, page, head_dim // group, 2)

@@ -50,6 +50,13 @@ def test_cache_refuses(i, change):
         D.KvCache(*tensors)
 
 
+@pytest.mark.parametrize("args", [(0, 16, 1, 64, 64), (2, 24, 1, 64, 64), (2, 16, 0, 64, 64), (2, 16, 1, 80, 80),
+                                  (2, 16, 1, 64, 0), (2, 16, 1, 64, 48), (2, 16, 1, 64, 128)])
+def test_empty_cache_refuses(args):
+    with pytest.raises(L.OhipError):
+        D.KvCache.empty(*args)
+
+
 def test_cache_layout_of_the_reference():
     """Channel and token of every code, from the layout's description."""
     c = D.KvCache(*_cache(pages=2, page=32, kv=1, dim=64))
