@@ -360,18 +360,21 @@ hipError_t run_gemm_q4(int dtype, const Q4Args& g, const FloatOut& o, hipStream_
 // ------------------------------------------------------------------ many rows
 // The weight as K-contiguous rows of T (ldw elements, zeros past K) for the
 // MFMA engine: s * (c - z) in f32, rounded once.
+// Four lanes write 64 bytes of a row (4096 x 22016 f16 88 us, 2.6 TB/s; in the
+// codes' order, a row a lane, 95): a tenth of the product that follows for a
+// few thousand rows.
 template <class T>
 __global__ void __launch_bounds__(256)
 q4_unpack_kernel(const u32x4* __restrict__ codes, const T* __restrict__ scales, const uint8_t* __restrict__ zp,
                  T* __restrict__ dst, int N, int K, int64_t ldw, int group, int kt, int64_t tiles) {
   const int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (tile >= tiles) return;
-  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int lane = threadIdx.x & 63, r = lane >> 2, q = lane & 3;   // four lanes write a row's 32 k
   const int64_t n16 = tile / kt;
   const int k0 = (int)(tile % kt) * 128, blocks = (K + group - 1) / group;
   const int64_t n = n16 * 16 + r;
   if (n >= N) return;
-  const u32x4 w = codes[tile * 64 + lane];
+  const u32x4 w = codes[tile * 64 + 16 * q + r];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
     const int k = k0 + 32 * s + 8 * q;
