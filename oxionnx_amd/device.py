@@ -68,6 +68,7 @@ _ATTN_PREFILL = _Packer("@3q6if4q", L.AttnPrefillDesc)
 # the zero points that one byte can hold, for calls with a single one
 _ZERO_POINTS = np.arange(-128, 256, dtype=np.int32)
 _ZERO_POINTS_AT = _ZERO_POINTS.ctypes.data
+_TYPE_NAMES = {"f32": L.F32, "f16": L.F16, "bf16": L.BF16}
 
 
 def _out_dim(size, pad_begin, pad_end, k, dil, stride):
@@ -305,8 +306,9 @@ class HipContext:
 
     def weight_q4(self, codes, scales, zero_points=None, k=None, dtype=None, name=None, label="Gemm.B4"):
         """A weight [K, N] of 4-bit codes (ohip_weight_q4): codes uint8 [N, blocks, group / 2], scales [N, blocks]
-        (float32 or float16, rounded to `dtype`, the activations' type, by default their own), zero_points uint8
-        [N, ceil(blocks / 2)] or None (8 everywhere); k if K does not fill the last block."""
+        (float32, float16, or bfloat16 as its 16 bits, rounded to `dtype`), zero_points uint8 [N, ceil(blocks / 2)]
+        or None (8 everywhere); dtype: the activations' type (L.F32 / F16 / BF16 or "f32" / "f16" / "bf16"), by
+        default the scales' own; k if K does not fill the last block."""
         codes, scales = np.ascontiguousarray(codes), np.asarray(scales)
         if codes.ndim != 3 or codes.dtype != np.uint8 or scales.shape != codes.shape[:2]:
             raise _invalid("weight_q4: codes uint8 [N, blocks, group / 2] and scales [N, blocks]")
@@ -314,16 +316,23 @@ class HipContext:
         k = blocks * 2 * half if k is None else k
         if not blocks or not half or (k + 2 * half - 1) // (2 * half) != blocks:
             raise _invalid("weight_q4: K does not end in the last block")
-        dtype = (L.F16 if scales.dtype == np.float16 else L.F32) if dtype is None else dtype
+        bits = scales.dtype in (np.uint16, np.int16)   # numpy has no bfloat16
+        if dtype is None:
+            dtype = L.BF16 if bits else L.F16 if scales.dtype == np.float16 else L.F32
+        dtype = _TYPE_NAMES.get(dtype, dtype)
+        if dtype not in (L.F32, L.F16, L.BF16):
+            raise _invalid("weight_q4: dtype")
+        if bits and dtype != L.BF16:
+            scales = (scales.view(np.uint16).astype(np.uint32) << 16).view(np.float32)
         if dtype == L.F32:
             scales = np.ascontiguousarray(scales, np.float32)
         elif dtype == L.F16:
             scales = np.ascontiguousarray(scales, np.float16)
-        elif dtype == L.BF16:
+        elif bits:
+            scales = np.ascontiguousarray(scales)
+        else:
             torch = _torch()
             scales = torch.from_numpy(np.array(scales, np.float32)).to(torch.bfloat16).view(torch.int16).numpy()
-        else:
-            raise _invalid("weight_q4: dtype")
         if zero_points is not None:
             zero_points = np.ascontiguousarray(zero_points)
             if zero_points.dtype != np.uint8 or zero_points.shape != (n, (blocks + 1) // 2):
