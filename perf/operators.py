@@ -218,11 +218,9 @@ def prepare(case, seed):
     # What a serving program keeps: the context, packed weights, the cache's handle and output buffers.
     s["ctx"], kind = _ctx(), case["kind"]
     if kind == "q4":
-        from oxionnx_amd import _lib as L
-        codes, scales, zero_points = (None if t is None else t.cpu().numpy() for t in
-                                      (s["codes"], s["scales"].float(), s["zero_points"]))
-        s["w"] = s["ctx"].weight_q4(codes, scales, zero_points=zero_points, k=case["k"],
-                                    dtype={"f32": L.F32, "f16": L.F16, "bf16": L.BF16}[case["dtype"]])
+        host = [None if t is None else t.cpu().numpy() if t.dtype != torch.bfloat16 else t.view(torch.int16).cpu().numpy()
+                for t in (s["codes"], s["scales"], s["zero_points"])]
+        s["w"] = s["ctx"].weight_q4(host[0], host[1], zero_points=host[2], k=case["k"], dtype=case["dtype"])
         s["y"] = torch.empty((case["m"], case["n"]), dtype=s["a"].dtype, device="cuda")
     elif kind == "prefill":
         s["y"] = torch.empty(s["q"].shape, dtype=s["q"].dtype, device="cuda")
