@@ -107,6 +107,8 @@ def _heads(t, name, dtype, device):
     tokens, heads, dim = t.shape
     if (strides[2] != 1 and dim > 1) or (strides[1] != dim and heads > 1):
         raise _invalid(f"{name}: a token's heads are not next to each other")
+    if tokens > 1 and strides[0] < heads * dim:   # (a stride of 0, an expanded tensor's, is the library's "packed")
+        raise _invalid(f"{name}: tokens share memory")
     return strides[0] if tokens > 1 else heads * dim
 
 
@@ -522,6 +524,8 @@ class HipContext:
         if (a.get_device() != at or out.get_device() != at or out.dtype != a.dtype or out.shape != (m, n)
                 or (k > 1 and a.stride(1) != 1) or (n > 1 and out.stride(1) != 1)):
             raise _invalid("gemm_q4: a [M, K] and out [M, N] of one type on the context's GPU, rows contiguous")
+        if m > 1 and (a.stride(0) < k or out.stride(0) < n):   # (a stride of 0 is the library's "packed")
+            raise _invalid("gemm_q4: rows share memory")
         if bias is not None and (bias.dtype != a.dtype or bias.get_device() != at or not bias.is_contiguous()
                                  or bias.numel() != n):
             raise _invalid("gemm_q4: bias [N] of the activations' type")

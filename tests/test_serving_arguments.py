@@ -51,3 +51,71 @@ def test_weight_type_by_default(monkeypatch):
         assert rec.calls[-1][3] == code
     with pytest.raises(L.OhipError):
         D.HipContext.weight_q4(rec, codes, np.ones((2, 1), np.float32), dtype="f64")
+
+
+class _Context:
+    """A HipContext of tensors on the host; its library must not be reached."""
+    h, device = None, -1
+    gemm_q4, kv_append = D.HipContext.gemm_q4, D.HipContext.kv_append
+    attn_decode, attn_prefill = D.HipContext.attn_decode, D.HipContext.attn_prefill
+
+
+@pytest.fixture
+def host_ctx(monkeypatch):
+    def raw(name):
+        raise AssertionError(f"{name} was reached")
+    monkeypatch.setattr(L, "raw", raw)
+    return _Context()
+
+
+def _ints(*shape):
+    return torch.zeros(shape, dtype=torch.int32)
+
+
+def _cache():
+    params = (3, 2, 16, 2, 2)
+    return D.KvCache(torch.zeros((3, 2, 16, 4, 2, 4), dtype=torch.uint8), torch.zeros((3, 2, 1, 16, 16, 2), dtype=torch.uint8),
+                     torch.zeros(params, dtype=torch.float16), torch.zeros(params, dtype=torch.float16))
+
+
+def _rows(tokens, heads, shared):
+    """[tokens, heads, 64] of which (shared) all tokens are one, or neighbours overlap."""
+    if shared == "expanded":
+        return torch.zeros((1, heads, 64), dtype=torch.float16).expand(tokens, heads, 64)
+    if shared == "overlapping":
+        return torch.zeros(tokens * 64 * heads, dtype=torch.float16).as_strided((tokens, heads, 64), (8, 64, 1))
+    return torch.zeros((tokens, heads, 64), dtype=torch.float16)
+
+
+@pytest.mark.parametrize("shared", ["expanded", "overlapping"])
+@pytest.mark.parametrize("at", ["a", "out"])
+def test_product_refuses_rows_that_share_memory(host_ctx, shared, at):
+    class _Weight:
+        shape, handle = (64, 64), None
+    t = {"a": _rows(8, 1, None)[:, 0], "out": _rows(8, 1, None)[:, 0], at: _rows(8, 1, shared)[:, 0]}
+    with pytest.raises(L.OhipError):
+        host_ctx.gemm_q4(t["a"], _Weight(), out=t["out"])
+
+
+@pytest.mark.parametrize("shared", ["expanded", "overlapping"])
+@pytest.mark.parametrize("at", ["q", "k", "v", "q_out", "k_out", "v_out"])
+def test_append_refuses_tokens_that_share_memory(host_ctx, shared, at):
+    t = {n: _rows(8, 4 if n[0] == "q" else 2, shared if n == at else None) for n in ("q", "k", "v", "q_out", "k_out", "v_out")}
+    with pytest.raises(L.OhipError):
+        host_ctx.kv_append(_cache(), t.pop("k"), t.pop("v"), _ints(8), **t)
+
+
+@pytest.mark.parametrize("shared", ["expanded", "overlapping"])
+@pytest.mark.parametrize("at", ["q", "k", "v", "out"])
+def test_attention_refuses_tokens_that_share_memory(host_ctx, shared, at):
+    t = {n: _rows(8, 2 if n in "kv" else 4, shared if n == at else None) for n in ("q", "k", "v", "out")}
+    with pytest.raises(L.OhipError):
+        host_ctx.attn_prefill(t["q"], t["k"], t["v"], _ints(2), out=t["out"])
+    if at in ("q", "out"):
+        with pytest.raises(L.OhipError):
+            host_ctx.attn_decode(t["q"], _cache(), _ints(8, 1), _ints(8), out=t["out"])
+
+
+def test_tokens_of_one_row_may_have_any_stride():
+    assert D._heads(torch.zeros((1, 4, 64), dtype=torch.float16).expand(1, 4, 64), "q", torch.float16, -1) == 256
+    assert D._heads(torch.zeros((5, 300), dtype=torch.float16)[:, :256].view(5, 4, 64), "q", torch.float16, -1) == 300
