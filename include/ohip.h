@@ -362,8 +362,10 @@ int ohip_weight_q4(ohip_ctx* ctx, const ohip_weight_key* key, const uint8_t* cod
                    int dtype, const void* scales, const uint8_t* zero_points, ohip_weight** out);
 /* Y[M,N] = act(A B + bias), B of ohip_weight_q4, A / bias [N] (may be NULL) /
  * Y of `dtype`.  Up to 64 rows the codes are multiplied as they are (exact
- * products, f32 sums by group); more rows unpack B to `dtype` (each value
- * rounded once) into a pool buffer for the MFMA engine. */
+ * products, f32 sums by group that the scale then multiplies; of BF16 these
+ * sums pass through up to 143 times the activations, unless that is not
+ * finite); more rows unpack B to `dtype` (each value rounded once) into a
+ * pool buffer for the MFMA engine. */
 typedef struct {
     int64_t m, k, n;
     int dtype;

@@ -77,8 +77,8 @@ template <> struct Act<float> { float v[8]; };
 
 // The sixteen-column product of one word of codes with activations, exact
 // codes: f16 takes the bias off each code (exact); bf16 adds a second product
-// with -(bias + z); f32 runs the f32 instruction, element e of every lane a
-// k of its own.
+// with -(bias + z) (Q4Exact where that leaves f32); f32 runs the f32
+// instruction, element e of every lane a k of its own.
 template <class T> struct Q4Mma;
 template <> struct Q4Mma<_Float16> {
   u32x4 off;   // (1024 + z) twice, (64 + z) twice
@@ -104,6 +104,19 @@ template <> struct Q4Mma<__bf16> {
   __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const {
     return mma16<__bf16>(f, a.v, mma16<__bf16>(off, a.v, c));
   }
+};
+// c - z itself, exact in bf16 too: what finite sums do without, since each
+// element costs a conversion.
+struct Q4Exact {
+  int z;
+  __device__ __forceinline__ void zero(int zp) { z = zp; }
+  __device__ __forceinline__ u32x4 frag(uint32_t w) const {
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (float)((int)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z);
+    return u32x4{pack2<__bf16>(e[0], e[1]), pack2<__bf16>(e[2], e[3]), pack2<__bf16>(e[4], e[5]), pack2<__bf16>(e[6], e[7])};
+  }
+  __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const { return mma16<__bf16>(f, a.v, c); }
 };
 template <> struct Q4Mma<float> {
   int z;
@@ -239,10 +252,9 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
                        __builtin_assume_aligned(row + (((kPer * (4 * s + q) + j) ^ r) * 16), 16), 16);
     return x;
   };
-  auto sum = [&](const Tile& f, auto act) __attribute__((always_inline)) {
+  auto sum = [&](auto mul, const Tile& f, auto act) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < GN; ++g) {
-      Q4Mma<T> mul;
       mul.zero(f.z[g]);
       f32x4 raw[TM];
 #pragma unroll
@@ -283,8 +295,27 @@ q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes,
       }
       if (i + k + kRing - 1 < mine) load(ring[(k + kRing - 1) % kRing], i + k + kRing - 1);
       if constexpr (STAGE) arrived(i + k + kRing - 1 < mine);
-      if constexpr (STAGE) sum(ring[k], [&](int s, int t) __attribute__((always_inline)) { return staged(k, s, t); });
-      else sum(ring[k], [&](int s, int t) __attribute__((always_inline)) { return acts[k % kActs].x[s][t]; });
+      if constexpr (STAGE) sum(Q4Mma<T>(), ring[k], [&](int s, int t) __attribute__((always_inline)) { return staged(k, s, t); });
+      else sum(Q4Mma<T>(), ring[k], [&](int s, int t) __attribute__((always_inline)) { return acts[k % kActs].x[s][t]; });
+    }
+  }
+  if constexpr (std::is_same<T, __bf16>::value) {
+    // An infinity, or a number whose product with the codes' bias is beyond
+    // f32, has left inf - inf: such a wave takes its sums again.
+    float finite = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4 * TM; ++i) finite = __builtin_fmaf(acc[i / 4][i % 4], 0.0f, finite);
+    if (__any(finite != 0.0f)) {
+#pragma unroll
+      for (int t = 0; t < TM; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+      for (int i = 0; i < mine; ++i) {
+        Tile f;
+        Acts x;
+        load(f, i);
+        load_acts(x, i);
+        sum(Q4Exact(), f, [&](int s, int t) __attribute__((always_inline)) { return x.x[s][t]; });
+      }
     }
   }
 #pragma unroll
