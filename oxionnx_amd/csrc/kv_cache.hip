@@ -139,6 +139,9 @@ kv_append_kernel(const KvAppendArgs p) {
         hi = __builtin_fmaxf(hi, dpp<kMirror16>(hi));
       }
       const uint64_t any = __ballot(bad);
+      // (finite, so that a group of nothing but one infinity has no extent)
+      lo = __builtin_fminf(__builtin_fmaxf(lo, -__FLT_MAX__), __FLT_MAX__);
+      hi = __builtin_fminf(__builtin_fmaxf(hi, -__FLT_MAX__), __FLT_MAX__);
       if (any && ((any >> (threadIdx.x & 63 & ~(gl - 1))) & ((1u << gl) - 1))) lo = hi = __builtin_nanf("");
       const _Float16 s16 = (_Float16)finite_f16((hi - lo) * (1.0f / 15.0f)), l16 = (_Float16)finite_f16(lo);
       const float sc = (float)s16, lw = (float)l16;

@@ -69,3 +69,29 @@ def test_q4_infinite_and_huge_activations(ctx, dtype, m, k, group, zp):
     near = finite & (want.abs() + bound < limit)   # (the others may round to infinity)
     assert ((got - want).abs() <= bound)[near].all()
     assert near.any() or m == 1
+
+
+# ------------------------------------------------------------------ append
+@pytest.mark.parametrize("dtype", HALF, ids=["f16", "bf16"])
+@pytest.mark.parametrize("dim,group", [(64, 32), (128, 64), (128, 128)])
+def test_append_groups_of_infinities(ctx, dtype, dim, group):
+    """A group of one infinity alone is held as f16's largest number of its sign, one of both from end to end; only a NaN
+    makes a group NaN."""
+    inf = float("inf")
+    cache = ctx.kv_cache(1, 16, 1, dim, group)
+    v = torch.zeros((5, 1, dim), dtype=dtype)
+    v[0], v[1] = inf, -inf
+    v[2], v[2, 0, 1::2] = inf, -inf
+    v[3], v[3, 0, 1::2] = inf, float("nan")
+    v[4, 0, :group], v[4, 0, group:] = -inf, 1.0
+    k, got = ctx.kv_append(cache, v.cuda(), v.cuda(), torch.arange(5, dtype=torch.int32).cuda())[1:]
+    kc, vc, kp, vp = R.read_cache(cache)
+    for codes, p, out in ((kc, kp, k), (vc, vp, got)):
+        low, high = 65504.0, 15 * 65504.0 - 65504.0   # f16's largest; lowest and largest step from minus it
+        held = R.values(codes, p)[0, 0]
+        assert (held[0] == low).all() and (held[1] == -low).all()
+        assert (held[2, ::2] == high).all() and (held[2, 1::2] == -low).all()
+        assert held[3].isnan().all()
+        assert (held[4, :group] == -low).all() and (held[4, group:] == 1).all()
+        for i in range(5):
+            np.testing.assert_array_equal(R.f64(out)[i, 0].numpy(), R.f64(held[i].float().to(dtype)).numpy())
