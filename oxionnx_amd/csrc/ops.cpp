@@ -2574,7 +2574,9 @@ extern "C" int ohip_attn_prefill(ohip_ctx* ctx, const ohip_attn_prefill_desc* d,
   if (p.ldk > (1 << 22) || p.ldv > (1 << 22)) return fail(OHIP_DECLINED, "ohip_attn_prefill: rows too far apart");
   p.cu_q = cu_q; p.cu_k = cu_k; p.q_tokens = d->q_tokens; p.k_tokens = d->k_tokens;
   p.seqs = (int)d->seqs; p.kv = d->kv_heads; p.g = d->heads / d->kv_heads; p.dim = d->head_dim;
-  p.causal = d->causal != 0; p.window = d->window; p.c = d->scale * 1.4426950408889634f;
+  // (a window of all keys is none: the kernel subtracts it from places in 32 bits)
+  p.causal = d->causal != 0; p.window = d->window < d->q_tokens + d->k_tokens ? d->window : 0;
+  p.c = d->scale * 1.4426950408889634f;
   std::lock_guard<std::mutex> lock(ctx->mu);
   ctx->counters.dispatches++;
   hipError_t e = run_attn_prefill(d->dtype, p, ctx->stream);

@@ -95,3 +95,24 @@ def test_append_groups_of_infinities(ctx, dtype, dim, group):
         assert (held[4, :group] == -low).all() and (held[4, group:] == 1).all()
         for i in range(5):
             np.testing.assert_array_equal(R.f64(out)[i, 0].numpy(), R.f64(held[i].float().to(dtype)).numpy())
+
+
+# ------------------------------------------------------------------ prompt attention
+def offsets(lens):
+    return torch.tensor([0] + list(np.cumsum(lens)), dtype=torch.int32)
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=["f16", "bf16"])
+@pytest.mark.parametrize("nq,nk,causal", [([10], [100], False), ([140, 33], [130, 33], True), ([300], [300], True),
+                                          ([70], [5], False), ([200, 1], [90, 400], True)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 200, 700])
+def test_prefill_windows_of_everything(ctx, dtype, nq, nk, causal, window):
+    """Windows larger than any sequence, up to the type's largest, are none."""
+    kv, g, dim = 1, 2, 64
+    cu_q, cu_k = offsets(nq), offsets(nk)
+    q = normal(51, (int(cu_q[-1]), kv * g, dim), dtype)
+    k, v = (normal(52 + i, (int(cu_k[-1]), kv, dim), dtype) for i in range(2))
+    got = ctx.attn_prefill(q.cuda(), k.cuda(), v.cuda(), cu_q.cuda(), cu_k.cuda(), causal=causal, window=window)
+    R.close(got, R.prefill(q, k, v, cu_q, cu_k, dim ** -0.5, causal, window))
+    none = ctx.attn_prefill(q.cuda(), k.cuda(), v.cuda(), cu_q.cuda(), cu_k.cuda(), causal=causal)
+    assert torch.equal(got, none)
