@@ -564,6 +564,8 @@ class HipContext:
             elif q_out.shape != qshape:
                 raise _invalid("kv_append: q_out has another shape than q")
             ldqo, qp, qop = _heads(q_out, "kv_append: q_out", dt, at), q.data_ptr(), q_out.data_ptr()
+        elif q_out is not None:
+            raise _invalid("kv_append: q_out without q")
         if k_out is None:
             k_out = _torch().empty(shape, dtype=dt, device=k.device)
         if k_out is not False:
@@ -577,6 +579,8 @@ class HipContext:
                 raise _invalid("kv_append: v_out has another shape than k")
             ldvo, vop = _heads(v_out, "kv_append: v_out", dt, at), v_out.data_ptr()
         i32 = _TORCH_DT[L.I32]
+        if (cos is None) != (sin is None) or (cos is not None and positions is None):
+            raise _invalid("kv_append: cos, sin and positions come together")
         if cos is not None:
             f32, angles = _TORCH_DT[L.F32], cos.shape
             if len(angles) != 2:

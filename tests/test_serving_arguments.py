@@ -119,3 +119,11 @@ def test_attention_refuses_tokens_that_share_memory(host_ctx, shared, at):
 def test_tokens_of_one_row_may_have_any_stride():
     assert D._heads(torch.zeros((1, 4, 64), dtype=torch.float16).expand(1, 4, 64), "q", torch.float16, -1) == 256
     assert D._heads(torch.zeros((5, 300), dtype=torch.float16)[:, :256].view(5, 4, 64), "q", torch.float16, -1) == 300
+
+
+def test_append_refuses_half_of_a_rotation_and_of_queries(host_ctx):
+    k, angles, at = _rows(8, 2, None), torch.zeros((4, 32)), _ints(8)
+    for kw in ({"cos": angles, "sin": angles}, {"cos": angles, "positions": at}, {"sin": angles, "positions": at},
+               {"sin": angles}, {"q_out": _rows(8, 4, None)}):
+        with pytest.raises(L.OhipError):
+            host_ctx.kv_append(_cache(), k, k, _ints(8), **kw)
