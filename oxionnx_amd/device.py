@@ -51,8 +51,12 @@ class _Packer:
             return self._pack(*values)
         except (struct.error, OverflowError):
             types = [t for _, t in self._desc._fields_]
-            return bytes(self._desc(*(ctypes.cast(v, t) if issubclass(t, ctypes._Pointer) else v
-                                      for v, t in zip(values, types))))
+            d = self._desc(*(ctypes.cast(v, t) if issubclass(t, ctypes._Pointer) else v
+                             for v, t in zip(values, types)))
+            for (name, t), v in zip(self._desc._fields_, values):   # ctypes would take an integer's low bits
+                if t in (ctypes.c_int, ctypes.c_int64) and getattr(d, name) != v:
+                    raise L.OhipError(L.E_INVALID, f"{name} = {v} is out of range")
+            return bytes(d)
 
 
 _GEMM = _Packer("@3q2i2f2i2f2q", L.GemmDesc)

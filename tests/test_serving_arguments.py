@@ -127,3 +127,24 @@ def test_append_refuses_half_of_a_rotation_and_of_queries(host_ctx):
                {"sin": angles}, {"q_out": _rows(8, 4, None)}):
         with pytest.raises(L.OhipError):
             host_ctx.kv_append(_cache(), k, k, _ints(8), **kw)
+
+
+@pytest.mark.parametrize("window", [2 ** 31, 2 ** 32 + 5, -2 ** 31 - 1, 2 ** 63])
+def test_windows_beyond_the_descriptor_are_refused(host_ctx, window):
+    """(their low bits would be another window)"""
+    q = _rows(8, 4, None)
+    with pytest.raises(L.OhipError):
+        host_ctx.attn_prefill(q, q, q, _ints(2), window=window)
+    with pytest.raises(L.OhipError):
+        host_ctx.attn_decode(q, _cache(), _ints(8, 1), _ints(8), window=window)
+
+
+def test_integers_beyond_a_descriptor_are_refused():
+    for packer in (D._GEMM, D._CONV, D._CONVT, D._MATMUL, D._GEMM_Q4, D._KV_CACHE, D._KV_APPEND, D._ATTN_DECODE, D._ATTN_PREFILL):
+        fields = packer._desc._fields_
+        for i, (_, t) in enumerate(fields):
+            if t in (ctypes.c_int, ctypes.c_int64):
+                bits = 8 * ctypes.sizeof(t)
+                for v in (2 ** (bits - 1), -2 ** (bits - 1) - 1, 2 ** bits + 1):
+                    with pytest.raises(L.OhipError):
+                        packer(*(v if j == i else 1 for j in range(len(fields))))
