@@ -86,7 +86,12 @@ int ohip_sync(ohip_ctx* ctx);
  * buffers, so the caller keeps the captured inputs and outputs alive and
  * refills / reads them around ohip_graph_launch.  ohip_pool_parking(ctx, 1)
  * parks buffers without a capture (a dry run that leaves every buffer the
- * forward needs in the pool); ohip_pool_parking(ctx, 0) releases them. */
+ * forward needs in the pool); ohip_pool_parking(ctx, 0) releases them.
+ * A capture that somebody else opened on the context's stream is recorded
+ * alike.  The context does not know when that graph ends: the scratch that it
+ * holds, and device buffers freed while it was recorded, stay until the
+ * context is destroyed (later captures of that kind share them: replay them
+ * one after the other, on one stream). */
 typedef struct ohip_graph ohip_graph;
 int ohip_pool_parking(ohip_ctx* ctx, int on);
 int ohip_graph_begin(ohip_ctx* ctx);

@@ -109,6 +109,8 @@ struct DevPool {
   size_t held = 0;                           // bytes held from HIP
   bool parking = false;                      // freed buffers are parked, not reused
   std::vector<std::pair<void*, size_t>> parked;
+  std::atomic<bool> recording{false};        // an ohip_graph_begin is open
+  std::multimap<size_t, void*> captured;     // freed under a capture of someone else's: for such captures only
 };
 
 // The context's growable scratch.  A captured graph's kernels hold its address,
@@ -129,6 +131,7 @@ struct ohip_ctx {
   int tile_override = 0;
   std::shared_ptr<ScratchBuf> scratch;
   size_t scratch_bytes = 0;
+  std::vector<std::shared_ptr<ScratchBuf>> captured_scratch;   // used under a capture of someone else's
   uint8_t* padtab = nullptr;  // 256 entries of 16 bytes: entry b is sixteen copies of byte b
   std::map<std::string, ohip_weight*> weights;
   std::vector<ohip_weight*> transients;  // freed with the context if never released
@@ -192,8 +195,27 @@ struct ScratchPlan {
   }
 };
 
+// Whether the context's stream is under a capture that ohip_graph_begin did
+// not open.  How long that graph lives is not known here, so the buffers that
+// its kernels hold are kept until the context goes: the scratch, and pool
+// buffers freed meanwhile, which only such captures get again (one after the
+// other on one stream, like the scratch).
+static bool foreign_capture(ohip_ctx* ctx) {
+  if (ctx->pool.recording) return false;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(ctx->stream, &status) != hipSuccess) {
+    (void)hipGetLastError();
+    return false;
+  }
+  return status == hipStreamCaptureStatusActive;
+}
+
 static int scratch_reserve(ohip_ctx* ctx, size_t bytes) {
-  if (bytes <= ctx->scratch_bytes) return OHIP_OK;
+  if (bytes <= ctx->scratch_bytes) {
+    if (bytes && (ctx->captured_scratch.empty() || ctx->captured_scratch.back() != ctx->scratch) && foreign_capture(ctx))
+      ctx->captured_scratch.push_back(ctx->scratch);
+    return OHIP_OK;
+  }
   HIP_TRY(hipStreamSynchronize(ctx->stream), "hipStreamSynchronize");
   ctx->scratch.reset();
   ctx->scratch_bytes = 0;
@@ -362,6 +384,7 @@ extern "C" void ohip_ctx_destroy(ohip_ctx* ctx) {
   for (auto& kv : ctx->tables) (void)hipFree(kv.second);
   for (auto& kv : ctx->consts) (void)hipFree(kv.second);
   for (auto& kv : ctx->pool.free_blocks) (void)hipFree(kv.second);
+  for (auto& kv : ctx->pool.captured) (void)hipFree(kv.second);
   for (auto& kv : ctx->pool.live) (void)hipFree(kv.first);
   if (ctx->own) (void)hipStreamDestroy(ctx->own);
   delete ctx;
@@ -400,11 +423,19 @@ static size_t pool_class(size_t bytes) {
 static int pool_alloc(ohip_ctx* ctx, size_t bytes, void** p) {
   const size_t cap = pool_class(bytes);
   std::lock_guard<std::mutex> lock(ctx->pool_mu);
-  auto it = ctx->pool.free_blocks.lower_bound(cap);
-  if (it != ctx->pool.free_blocks.end() && it->first <= 2 * cap) {
+  auto* from = &ctx->pool.free_blocks;
+  auto it = from->lower_bound(cap);
+  if (!ctx->pool.captured.empty() && foreign_capture(ctx)) {   // the smaller of both, as one pool would give it
+    auto c = ctx->pool.captured.lower_bound(cap);
+    if (c != ctx->pool.captured.end() && (it == from->end() || c->first <= it->first)) {
+      from = &ctx->pool.captured;
+      it = c;
+    }
+  }
+  if (it != from->end() && it->first <= 2 * cap) {
     *p = it->second;
     ctx->pool.live[*p] = it->first;
-    ctx->pool.free_blocks.erase(it);
+    from->erase(it);
     return OHIP_OK;
   }
   hipError_t e = dev_malloc(ctx, p, cap);
@@ -426,7 +457,8 @@ static int pool_free(ohip_ctx* ctx, void* p) {
   std::lock_guard<std::mutex> lock(ctx->pool_mu);
   auto it = ctx->pool.live.find(p);
   if (it == ctx->pool.live.end()) return fail(OHIP_E_INVALID, "ohip_free: not a buffer of this context");
-  if (ctx->pool.parking) ctx->pool.parked.emplace_back(p, it->second);
+  if (foreign_capture(ctx)) ctx->pool.captured.emplace(it->second, p);
+  else if (ctx->pool.parking) ctx->pool.parked.emplace_back(p, it->second);
   else ctx->pool.free_blocks.emplace(it->second, p);
   ctx->pool.live.erase(it);
   return OHIP_OK;
@@ -464,12 +496,12 @@ extern "C" int ohip_graph_begin(ohip_ctx* ctx) {
   {
     std::lock_guard<std::mutex> lock(ctx->pool_mu);
     unpark_all(ctx, ctx->pool.parked);
-    ctx->pool.parking = true;
+    ctx->pool.parking = ctx->pool.recording = true;
   }
   hipError_t e = hipStreamBeginCapture(ctx->stream, hipStreamCaptureModeRelaxed);
   if (e != hipSuccess) {
     std::lock_guard<std::mutex> lock(ctx->pool_mu);
-    ctx->pool.parking = false;
+    ctx->pool.parking = ctx->pool.recording = false;
     return hip_fail(e, "hipStreamBeginCapture");
   }
   return OHIP_OK;
@@ -488,7 +520,7 @@ extern "C" int ohip_graph_end(ohip_ctx* ctx, ohip_graph** out) {
   hipError_t e = hipStreamEndCapture(ctx->stream, &g->graph);
   {
     std::lock_guard<std::mutex> lock(ctx->pool_mu);
-    ctx->pool.parking = false;
+    ctx->pool.parking = ctx->pool.recording = false;
     g->held.swap(ctx->pool.parked);
   }
   if (e == hipSuccess) e = hipGraphInstantiate(&g->exec, g->graph, nullptr, nullptr, 0);
