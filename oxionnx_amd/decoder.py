@@ -93,7 +93,14 @@ class DecoderLayer:
         return x + self.ctx.gemm_q4((torch.nn.functional.silu(gate.float()) * up.float()).to(x.dtype), self.down)
 
     def prefill(self, x, cu, slots, positions):
-        """Whole prompts, packed: x [tokens, hidden], offsets cu [sequences + 1]."""
+        """Whole prompts, packed: x [tokens, hidden], offsets cu [sequences + 1].  They begin at position 0: attention
+        over prompts does not read the cache, so a sequence that holds tokens already is refused (a capture cannot look
+        at the positions: there the caller sees to it)."""
+        import torch
+        if x.shape[0] and not (positions.is_cuda and torch.cuda.is_current_stream_capturing()):
+            first = cu[:-1][cu[1:] > cu[:-1]].long()
+            if positions[first].any():
+                raise L.OhipError(L.E_INVALID, "prefill: a sequence holds tokens already")
         q, k, v = self._append(x, slots, positions)
         return self._rest(x, self.ctx.attn_prefill(q, k, v, cu))
 
