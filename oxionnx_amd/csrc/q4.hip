@@ -151,11 +151,13 @@ template <class T, int TM, int NW> constexpr int q4_slots() {
 // of it is 64 lookups of 16 bytes.  STAGE copies them into LDS instead, 64
 // bytes a lookup, and reads the fragments there (16 x 11008 x 4096 bf16 14.5 ->
 // 9.8 us, 64 rows 46 -> 21).  A ring of tiles of 128 k of codes and of
-// activations is in flight.
+// activations is in flight.  (The waits for LDS count the loads behind them,
+// which therefore go through plain pointers: loads of __restrict__ ones the
+// compiler may move across the waits.)
 template <class T, int TM, int GS, int NW, bool STAGE>
 __global__ void __launch_bounds__(64 * NW, NW / 4)
-q4_kernel(const T* __restrict__ a, int64_t lda, const u32x4* __restrict__ codes, const T* __restrict__ scales,
-          const uint8_t* __restrict__ zp, int M, int N, int K, int group, const FloatEpi<T> epi) {
+q4_kernel(const T* a, int64_t lda, const u32x4* codes, const T* scales, const uint8_t* zp, int M, int N, int K, int group,
+          const FloatEpi<T> epi) {
   __shared__ f32x4 red[NW][TM][64];
   constexpr int GN = 4 / GS;   // groups of a tile
   // (what the registers hold: a tile of activations is 16 TM registers of f16, 32 of f32)
