@@ -77,8 +77,8 @@ template <> struct Act<float> { float v[8]; };
 
 // The sixteen-column product of one word of codes with activations, exact
 // codes: f16 takes the bias off each code (exact); bf16 adds a second product
-// with -(bias + z) (Q4Exact where that leaves f32); f32 runs the f32
-// instruction, element e of every lane a k of its own.
+// with -(bias + z) (q4_kernel takes sums again where that leaves f32); f32
+// runs the f32 instruction, element e of every lane a k of its own.
 template <class T> struct Q4Mma;
 template <> struct Q4Mma<_Float16> {
   u32x4 off;   // (1024 + z) twice, (64 + z) twice
@@ -104,19 +104,6 @@ template <> struct Q4Mma<__bf16> {
   __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const {
     return mma16<__bf16>(f, a.v, mma16<__bf16>(off, a.v, c));
   }
-};
-// c - z itself, exact in bf16 too: what finite sums do without, since each
-// element costs a conversion.
-struct Q4Exact {
-  int z;
-  __device__ __forceinline__ void zero(int zp) { z = zp; }
-  __device__ __forceinline__ u32x4 frag(uint32_t w) const {
-    float e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = (float)((int)((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u) - z);
-    return u32x4{pack2<__bf16>(e[0], e[1]), pack2<__bf16>(e[2], e[3]), pack2<__bf16>(e[4], e[5]), pack2<__bf16>(e[6], e[7])};
-  }
-  __device__ __forceinline__ f32x4 mma(u32x4 f, const Act<__bf16>& a, f32x4 c) const { return mma16<__bf16>(f, a.v, c); }
 };
 template <> struct Q4Mma<float> {
   int z;
@@ -150,14 +137,22 @@ template <class T, int TM, int NW> constexpr int q4_slots() {
 // CU's cache: a fragment's neighbouring lanes are of different rows, so a load
 // of it is 64 lookups of 16 bytes.  STAGE copies them into LDS instead, 64
 // bytes a lookup, and reads the fragments there (16 x 11008 x 4096 bf16 14.5 ->
-// 9.8 us, 64 rows 46 -> 21).  A ring of tiles of 128 k of codes and of
-// activations is in flight.  (The waits for LDS count the loads behind them,
-// which therefore go through plain pointers: loads of __restrict__ ones the
-// compiler may move across the waits.)
+// 9.7 us, 64 rows 46 -> 21.5).  A ring of tiles of 128 k of codes and of
+// activations is loaded ahead.  As compiled most tiles wait for all loads in
+// flight all the same, the newest among them: the zero points' branch and the
+// conditional prefetch join paths of different counts, and scales are unpacked
+// next to their load.  So a deeper ring gains nothing.  (The waits for LDS
+// count the loads behind them, which therefore go through plain pointers:
+// loads of __restrict__ ones the compiler may move across the waits.)
 template <class T, int TM, int GS, int NW, bool STAGE>
 __global__ void __launch_bounds__(64 * NW, NW / 4)
-q4_kernel(const T* a, int64_t lda, const u32x4* codes, const T* scales, const uint8_t* zp, int M, int N, int K, int group,
-          const FloatEpi<T> epi) {
+q4_kernel(const Q4Args args, const FloatEpi<T> epi) {
+  const T* const a = static_cast<const T*>(args.a);
+  const u32x4* const codes = static_cast<const u32x4*>(args.codes);
+  const T* const scales = static_cast<const T*>(args.scales);
+  const uint8_t* const zp = args.zp;
+  const int64_t lda = args.lda;
+  const int M = args.M, N = args.N, K = args.K, group = args.group;
   __shared__ f32x4 red[NW][TM][64];
   constexpr int GN = 4 / GS;   // groups of a tile
   // (what the registers hold: a tile of activations is 16 TM registers of f16, 32 of f32)
@@ -254,9 +249,10 @@ q4_kernel(const T* a, int64_t lda, const u32x4* codes, const T* scales, const ui
                        __builtin_assume_aligned(row + (((kPer * (4 * s + q) + j) ^ r) * 16), 16), 16);
     return x;
   };
-  auto sum = [&](auto mul, const Tile& f, auto act) __attribute__((always_inline)) {
+  auto sum = [&](const Tile& f, auto act) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < GN; ++g) {
+      Q4Mma<T> mul;
       mul.zero(f.z[g]);
       f32x4 raw[TM];
 #pragma unroll
@@ -297,27 +293,8 @@ q4_kernel(const T* a, int64_t lda, const u32x4* codes, const T* scales, const ui
       }
       if (i + k + kRing - 1 < mine) load(ring[(k + kRing - 1) % kRing], i + k + kRing - 1);
       if constexpr (STAGE) arrived(i + k + kRing - 1 < mine);
-      if constexpr (STAGE) sum(Q4Mma<T>(), ring[k], [&](int s, int t) __attribute__((always_inline)) { return staged(k, s, t); });
-      else sum(Q4Mma<T>(), ring[k], [&](int s, int t) __attribute__((always_inline)) { return acts[k % kActs].x[s][t]; });
-    }
-  }
-  if constexpr (std::is_same<T, __bf16>::value) {
-    // An infinity, or a number whose product with the codes' bias is beyond
-    // f32, has left inf - inf: such a wave takes its sums again.
-    float finite = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4 * TM; ++i) finite = __builtin_fmaf(acc[i / 4][i % 4], 0.0f, finite);
-    if (__any(finite != 0.0f)) {
-#pragma unroll
-      for (int t = 0; t < TM; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-      for (int i = 0; i < mine; ++i) {
-        Tile f;
-        Acts x;
-        load(f, i);
-        load_acts(x, i);
-        sum(Q4Exact(), f, [&](int s, int t) __attribute__((always_inline)) { return x.x[s][t]; });
-      }
+      if constexpr (STAGE) sum(ring[k], [&](int s, int t) __attribute__((always_inline)) { return staged(k, s, t); });
+      else sum(ring[k], [&](int s, int t) __attribute__((always_inline)) { return acts[k % kActs].x[s][t]; });
     }
   }
 #pragma unroll
@@ -327,8 +304,46 @@ q4_kernel(const T* a, int64_t lda, const u32x4* codes, const T* scales, const ui
   f32x4 v = red[0][wave][lane];
 #pragma unroll
   for (int k = 1; k < NW; ++k) v += red[k][wave][lane];
-  const int i = blockIdx.x * 16 + 4 * q, j = wave * 16 + r;
-  if (j >= M || i >= N) return;
+  // The lane and the arguments anew: kept through the loop they cost it
+  // registers (64 rows x 11008 x 4096 bf16 23.8 us for 21.2).
+  uint64_t kernarg = (uint64_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm("" : "+s"(kernarg));
+  const auto& again = *reinterpret_cast<const __attribute__((address_space(4))) Q4Args*>(kernarg);   // (the first one)
+  const int M1 = TM > 2 ? again.M : M, N1 = TM > 2 ? again.N : N;   // (of few rows that load would be the last wait)
+  const int l1 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  const int r1 = l1 & 15, q1 = l1 >> 4, i = blockIdx.x * 16 + 4 * q1, j = wave * 16 + r1;
+  if constexpr (std::is_same<T, __bf16>::value) {
+    // An infinity, or a number whose product with the codes' bias is beyond
+    // f32, has left inf - inf: the wave takes its sums again, of all k, with
+    // c - z itself (exact in bf16 too, but a conversion each).
+    const f32x4 test = v * 0.0f;
+    if (__any(j < M1 && i < N1 && test[0] + test[1] + test[2] + test[3] != 0.0f)) {
+      const int K = again.K, kt = (K + 127) / 128, blocks = (K + again.group - 1) / again.group;
+      const T* x0 = static_cast<const T*>(again.a) + (int64_t)min(j, M1 - 1) * again.lda + 8 * q1;
+      const uint32_t* words = static_cast<const uint32_t*>(again.codes) + ((int64_t)blockIdx.x * kt * 64 + l1) * 4;
+      const T* s0 = static_cast<const T*>(again.scales) + (int64_t)blockIdx.x * blocks * 16 + 4 * q1;
+      const uint8_t* z0 = again.zp ? again.zp + (int64_t)blockIdx.x * blocks * 16 + r1 : nullptr;
+      v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+      for (int k = 0; k < K; k += 32) {
+        const int b = k / again.group * 16, z = z0 ? z0[b] : 8;
+        const uint32_t w = words[(int64_t)(k >> 7) * 256 + ((k >> 5) & 3)];
+        T c[8], x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          c[e] = (T)(float)((int)((w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15u) - z);
+          x[e] = k + 8 * q1 + e < K ? x0[k + e] : T(0);
+        }
+        u32x4 cf, xf;
+        __builtin_memcpy(&cf, c, 16);
+        __builtin_memcpy(&xf, x, 16);
+        const f32x4 raw = mma16<T>(cf, xf, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(to_f32(s0[b + e]), raw[e], v[e]);
+      }
+    }
+  }
+  if (j >= M1 || i >= N1) return;
   typename FloatEpi<T>::PreI pi;
   typename FloatEpi<T>::PreJ pj;
   epi.load_i(pi, i);
@@ -341,32 +356,31 @@ q4_kernel(const T* a, int64_t lda, const u32x4* codes, const T* scales, const ui
 
 template <class T, int TM, int NW, bool STAGE>
 static hipError_t q4_w(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
-  const T* a = static_cast<const T*>(g.a);
-  const u32x4* codes = static_cast<const u32x4*>(g.codes);
-  const T* sc = static_cast<const T*>(g.scales);
   const dim3 grid((unsigned)((g.N + 15) / 16)), block(64 * NW);
   if (g.group == 32)
-    hipLaunchKernelGGL((q4_kernel<T, TM, 1, NW, STAGE>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 1, NW, STAGE>), grid, block, 0, st, g, epi);
   else if (g.group == 64)
-    hipLaunchKernelGGL((q4_kernel<T, TM, 2, NW, STAGE>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 2, NW, STAGE>), grid, block, 0, st, g, epi);
   else
-    hipLaunchKernelGGL((q4_kernel<T, TM, 4, NW, STAGE>), grid, block, 0, st, a, g.lda, codes, sc, g.zp, g.M, g.N, g.K, g.group, epi);
+    hipLaunchKernelGGL((q4_kernel<T, TM, 4, NW, STAGE>), grid, block, 0, st, g, epi);
   return hipGetLastError();
 }
 template <class T, int TM, int NW> static hipError_t q4_s(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
   if constexpr (q4_slots<T, TM, NW>() > 0) {
     const int64_t bytes = ((g.M - 1) * g.lda + g.K) * (int64_t)sizeof(T);
     // Whole aligned chunks, which 32 bits address; of fewer rows most of a
-    // slot is filled for nothing (1 x 4096 x 11008 bf16 8.4 us, staged 9.1; 4
-    // rows 9.2 and 8.8; f32 4 rows 23.6 and 25.3, 8 rows 25.4 and 25.3).
+    // slot is filled for nothing (4096 x 11008 in groups of 128, bf16: 1 row
+    // 7.3 us, staged 7.8; 4 rows 8.5 and 7.8; f32: 4 rows 23.5 and 23.1, 8 rows
+    // 25.0 and 23.2).
     if (g.M > (sizeof(T) == 4 ? 4 : 2) && g.K * sizeof(T) % 16 == 0 && g.lda * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(g.a) % 16 == 0 && bytes < INT_MAX)
       return q4_w<T, TM, NW, true>(g, epi, st);
   }
   return q4_w<T, TM, NW, false>(g, epi, st);
 }
-// Four waves a block where there are two blocks a CU or more (1 x 4096 x 11008
-// bf16, 688 blocks, not staged: 8.4 us, eight waves 9.5; 32 rows 12.8 and 16.4), else
-// eight (16 x 11008 x 4096, 256 blocks, not staged: 14.8, four 17.5).
+// Four waves a block where there are two blocks a CU or more (4096 x 11008
+// bf16, 688 blocks: 1 row 7.3 us with either, 16 rows 8.0, eight waves 11.2, 32
+// rows 11.1 and 15.4), else eight (16 x 11008 x 4096, 256 blocks: 9.7, four
+// 14.8).
 template <class T, int TM> static hipError_t q4_t(const Q4Args& g, const FloatEpi<T>& epi, hipStream_t st) {
   if constexpr (TM * sizeof(T) <= 4)
     if (g.N >= 512 * 16) return q4_s<T, TM, 4>(g, epi, st);
