@@ -97,12 +97,26 @@ class DecoderLayer:
         over prompts does not read the cache, so a sequence that holds tokens already is refused (a capture cannot look
         at the positions: there the caller sees to it)."""
         import torch
+        ends = None
         if x.shape[0] and not (positions.is_cuda and torch.cuda.is_current_stream_capturing()):
-            first = cu[:-1][cu[1:] > cu[:-1]].long()
-            if positions[first].any():
-                raise L.OhipError(L.E_INVALID, "prefill: a sequence holds tokens already")
+            ends = torch.stack((cu[:-1], cu[1:], positions[cu[:-1].clamp(max=x.shape[0] - 1)]))
+            if ends.is_cuda:   # looked at when the layer is under way: the host does not wait for the stream here
+                ends = torch.empty(ends.shape, dtype=ends.dtype, pin_memory=True).copy_(ends, non_blocking=True)
+                there = torch.cuda.Event()
+                there.record()
+            else:
+                self._begin_at_0(ends)
         q, k, v = self._append(x, slots, positions)
-        return self._rest(x, self.ctx.attn_prefill(q, k, v, cu))
+        y = self._rest(x, self.ctx.attn_prefill(q, k, v, cu))
+        if ends is not None and positions.is_cuda:
+            there.synchronize()
+            self._begin_at_0(ends)
+        return y
+
+    @staticmethod
+    def _begin_at_0(ends):
+        if any(first and a < b for a, b, first in zip(*ends.tolist())):
+            raise L.OhipError(L.E_INVALID, "prefill: a sequence holds tokens already")
 
     def decode(self, x, table, lens, slots, positions):
         """One token a sequence: x [sequences, hidden]; lens count it."""

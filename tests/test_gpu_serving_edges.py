@@ -116,3 +116,26 @@ def test_prefill_windows_of_everything(ctx, dtype, nq, nk, causal, window):
     R.close(got, R.prefill(q, k, v, cu_q, cu_k, dim ** -0.5, causal, window))
     none = ctx.attn_prefill(q.cuda(), k.cuda(), v.cuda(), cu_q.cuda(), cu_k.cuda(), causal=causal)
     assert torch.equal(got, none)
+
+
+# ------------------------------------------------------------------ the layer
+def test_second_prompt_of_a_sequence_is_refused():
+    """Its first tokens are in the cache, which prompt attention does not read; other sequences' prompts go on."""
+    from oxionnx_amd import decoder
+    from oxionnx_amd.device import HipContext
+    ctx = HipContext(0)
+    try:
+        cache = ctx.kv_cache(20, 16, 2, 64, 32)
+        layer = decoder.random_layer(ctx, cache, 4, 160, 224, 64, group=32)
+        pages = decoder.Pages(cache, 3, 5)
+        x = normal(70, (30, 160), torch.float16).cuda()
+        for counts, held in (([7, 0, 12], False), ([0, 9, 0], False), ([4, 0, 0], True), ([0, 1, 3], True)):
+            cu = offsets(counts).cuda()
+            args = (x[:sum(counts)].contiguous(), cu, *pages.extend(counts))
+            if held:
+                with pytest.raises(L.OhipError):
+                    layer.prefill(*args)
+            else:
+                assert layer.prefill(*args).isfinite().all()
+    finally:
+        ctx.close()
