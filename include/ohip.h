@@ -425,7 +425,8 @@ int ohip_kv_append(ohip_ctx* ctx, const ohip_kv_append_desc* d, const ohip_kv_ca
  * lens[b] - 1 (window 0: all) of sequence b, whose token t is in page
  * table[b][t / page].  Query head h uses key head h / (heads / kv_heads).
  * A sequence without tokens gets zeros; a length beyond the table's
- * width * page is that.  F16 or BF16. */
+ * width * page is that.  Scores are f32 sums that pass through up to 143
+ * (F16: 1039) times the queries.  F16 or BF16. */
 typedef struct {
     int64_t batch;
     int dtype, heads, width, window;   /* width: page table entries a sequence */
@@ -439,12 +440,12 @@ int ohip_attn_decode(ohip_ctx* ctx, const ohip_attn_decode_desc* d, const ohip_k
  * cu_q[i + 1] - 1 and the key rows cu_k[i] .. cu_k[i + 1] - 1 (device arrays
  * of seqs + 1 ascending offsets).  Its last query stands at its last key:
  * query i of nq sees (causal) the keys up to i + nk - nq and (window > 0) at
- * most `window` of the last of these.  A query that sees no key gets zeros;
- * keys and values that it does not see do not reach it, be they NaN.
- * head_dim: a multiple of 8 up to 128; rows are 16-byte aligned, at most 2^22
- * elements apart, heads next to each other.  Weights are rounded to `dtype`
- * before the products with the values, like every operand of the matrix
- * units; sums are f32.  F16 or BF16. */
+ * most `window` of the last of these.  A query that sees no key, or whose
+ * scores are all -inf, gets zeros; keys and values that it does not see do
+ * not reach it, be they NaN.  head_dim: a multiple of 8 up to 128; rows are
+ * 16-byte aligned, at most 2^22 elements apart, heads next to each other.
+ * Weights are rounded to `dtype` before the products with the values, like
+ * every operand of the matrix units; sums are f32.  F16 or BF16. */
 typedef struct {
     int64_t q_tokens, k_tokens, seqs;
     int dtype, heads, kv_heads, head_dim, causal, window;

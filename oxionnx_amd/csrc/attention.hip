@@ -9,7 +9,10 @@ namespace ohip {
 // sum need one exchange between a lane and the one 32 further; O^T = V^T P^T
 // takes P as it lies in the registers: k index 8 h + j (h = lane / 32) stands
 // for key 4 h + j of a block of 8, then of the next, and V's fragments come
-// from LDS through the transposing read.
+// from LDS through the transposing read.  P is rounded to T for that: two
+// parts of it, as over the cache, would be half as many products again, and
+// the matrix unit is the bound; against 64 bits the outputs are off by 1.25 to
+// 1.4 times what f32 weights leave (rounding the output itself included).
 //
 // Bound: the matrix products, with about as many cycles of vector instructions
 // (two thirds of them the exponentials and their arguments), so each stage
@@ -17,11 +20,12 @@ namespace ohip {
 // neighbours.  Tiles are loaded straight into LDS a pass ahead; a CU has room
 // for two blocks, each of which works through the other's barriers, its first
 // tiles and its last rows.  32 heads, 8 of keys, of 128 channels: 8192 tokens
-// 535 us (1026 TFLOP/s, 75 % of a large matrix product's rate), seven prompts
-// of 8191 tokens 141, the last 1000 of 4000 within 2048 51.  Eight waves that
-// share a tile and load three passes ahead, one block a CU: 546, 153 and 71;
-// four of them 728, 222 and 60.  Blocks in the order of their keys, most
-// first, through all sequences: 536, 141, and 0.2 us more for a short prompt.
+// 527 us (1043 TFLOP/s, 76 % of a large matrix product's rate), seven prompts
+// of 8191 tokens 138, the last 1000 of 4000 within 2048 51.  In another run,
+// these at 535, 141 and 51: eight waves that share a tile and load three
+// passes ahead, one block a CU, 546, 153 and 71; four of them 728, 222 and
+// 60; blocks in the order of their keys, most first, through all sequences
+// 536, 141, and 0.2 us more for a short prompt.
 constexpr int kPrefillK = 64, kPrefillQ = 128;
 
 // Slot of 16-byte chunk c of a staged row r: rows of 16 (8) chunks, XOR with a

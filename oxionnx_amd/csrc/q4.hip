@@ -315,7 +315,8 @@ q4_kernel(const Q4Args args, const FloatEpi<T> epi) {
   if constexpr (std::is_same<T, __bf16>::value) {
     // An infinity, or a number whose product with the codes' bias is beyond
     // f32, has left inf - inf: the wave takes its sums again, of all k, with
-    // c - z itself (exact in bf16 too, but a conversion each).
+    // c - z itself (exact in bf16 too, but a conversion each).  One wave and no
+    // care for speed: a call with such a row takes 60 to 190 us.
     const f32x4 test = v * 0.0f;
     if (__any(j < M1 && i < N1 && test[0] + test[1] + test[2] + test[3] != 0.0f)) {
       const int K = again.K, kt = (K + 127) / 128, blocks = (K + again.group - 1) / again.group;
